@@ -489,6 +489,60 @@ int tgt_nll_loss_fwd(const void* d_log_probs, const int64_t* d_target, int64_t N
 int tgt_nll_loss_bwd(const int64_t* d_target, const void* d_dloss, const float* d_count, int64_t N, int C, int dtype, int64_t ignore_index,
                      void* d_dlog_probs, void* stream);
 
+/* ---- a pre-norm gated block -------------------------------------------------
+ * Root-mean-square norm, gated projections and linears with an epilogue, for layers of any width.  No counterpart in
+ * the reference (its layers have LayerNorm and a feed-forward block of one projection and a GELU,
+ * models/graphormer_dist_node_level.py:27-39,296-314); they stand beside tgt_add_layer_norm_*, tgt_linear_act_* and
+ * tgt_linear_*.
+ *
+ * act: TGT_ACT_NONE, TGT_ACT_GELU (exact erf form), TGT_ACT_RELU or TGT_ACT_SILU (u / (1 + exp(-u))).
+ * d_x: [N, in_features]; weights [out_features, in_features] (nn.Linear.weight); biases [out_features] or NULL;
+ * outputs [N, out_features]; all of `dtype` and at any address of that type; sums in float32.  N < 2^31. */
+#define TGT_ACT_NONE 0
+#define TGT_ACT_SILU 3
+/* h = act(x Wg^T + bg) * (x Wu^T + bu) */
+int tgt_gated_linear_fwd(const void* d_x, const void* d_Wg, const void* d_Wu, const void* d_bg, const void* d_bu, int64_t N,
+                         int in_features, int out_features, int dtype, int act, void* d_h, void* stream);
+/* The same on operands in 8 bits (OCP e4m3): a value is its code times the scale of its row of x or of a weight.
+ * in_features: a multiple of 16, d_x and the weights on 16-byte boundaries or not.  Biases and h are of `dtype`. */
+int tgt_gated_linear_8bit_fwd(const void* d_x, const float* d_x_scales, const void* d_Wg, const float* d_Wg_scales,
+                              const void* d_Wu, const float* d_Wu_scales, const void* d_bg, const void* d_bu, int64_t N,
+                              int in_features, int out_features, int dtype, int act, void* d_h, void* stream);
+/* Backward: d_dx [N, in_features] or NULL; d_dW: HOST array of the two weights' gradients, or NULL; d_db: HOST array of the
+ * two biases' gradients (entries may be NULL), or NULL.  x, the weights and the biases are the forward's: what the
+ * activation was taken of is formed again.  The sums over nodes are added in a fixed order (same inputs, same bits).
+ * d_workspace: as many bytes as asked for, 16-byte aligned, contents need no initialisation.  N = 0: gradients of zero. */
+int64_t tgt_gated_linear_bwd_workspace_bytes(int64_t N, int in_features, int out_features, int dtype);
+int tgt_gated_linear_bwd(const void* d_x, const void* d_Wg, const void* d_Wu, const void* d_bg, const void* d_bu,
+                         const void* d_dh, int64_t N, int in_features, int out_features, int dtype, int act, void* d_dx,
+                         void* const* d_dW, void* const* d_db, void* d_workspace, int64_t workspace_bytes, void* stream);
+/* y = act(x W^T + b) + residual; residual [N, out_features] or NULL (its gradient is dy itself) */
+int tgt_linear_epilogue_fwd(const void* d_x, const void* d_W, const void* d_b, const void* d_residual, int64_t N, int in_features,
+                            int out_features, int dtype, int act, void* d_y, void* stream);
+int tgt_linear_epilogue_8bit_fwd(const void* d_x, const float* d_x_scales, const void* d_W, const float* d_W_scales,
+                                 const void* d_b, const void* d_residual, int64_t N, int in_features, int out_features, int dtype,
+                                 int act, void* d_y, void* stream);
+int64_t tgt_linear_epilogue_bwd_workspace_bytes(int64_t N, int in_features, int out_features, int dtype, int act);
+int tgt_linear_epilogue_bwd(const void* d_x, const void* d_W, const void* d_b, const void* d_dy, int64_t N, int in_features,
+                            int out_features, int dtype, int act, void* d_dx, void* d_dW, void* d_db, void* d_workspace,
+                            int64_t workspace_bytes, void* stream);
+/* s = x (+ r), rounded to `dtype`; y = s / sqrt(mean(s^2) + eps) * weight.  d_sum: [N, C], NULL without a residual (s is x
+ * then); d_rstd: float32 [N] for the backward, may be NULL.  C <= 16384. */
+int tgt_add_rms_norm_fwd(const void* d_x, const void* d_r, const void* d_weight, int64_t N, int C, float eps, int dtype,
+                         void* d_sum, void* d_y, float* d_rstd, void* stream);
+/* The same with y in 8 bits: d_codes [N, C] OCP e4m3, d_scales float32 [N].  A row's scale is the smallest power of two that brings
+ * its largest magnitude to at most 448 (at least 2^-126; 1 for a row of zeros); a code is the nearest to y / scale, ties to
+ * even, an infinity or a NaN becomes the NaN code. */
+int tgt_add_rms_norm_8bit(const void* d_x, const void* d_r, const void* d_weight, int64_t N, int C, float eps, int dtype,
+                          void* d_sum, void* d_codes, float* d_scales, void* stream);
+/* Rows of any matrix in 8 bits, in the same way (weights, once) */
+int tgt_quantize_rows(const void* d_w, int64_t N, int C, int dtype, void* d_codes, float* d_scales, void* stream);
+/* ds = norm-backward(dy) (+ d_ds_extra when != NULL: the gradient that reaches s past the norm), dweight = sum over rows of
+ * dy * s * rstd, added in a fixed order.  d_workspace: 16-byte aligned.  N = 0: a dweight of zeros. */
+int64_t tgt_rms_norm_bwd_workspace_bytes(int64_t N, int C);
+int tgt_rms_norm_bwd(const void* d_s, const void* d_weight, const float* d_rstd, const void* d_dy, const void* d_ds_extra, int64_t N,
+                     int C, int dtype, void* d_ds, void* d_dweight, void* d_workspace, int64_t workspace_bytes, void* stream);
+
 /* ---- graph-level attention bias ---------------------------------------------
  * GraphAttnBias.forward (models/graphormer_graph_level.py:94-156), edge_type other than
  * 'multi_hop' (:148-150).  With S1 = s + 1 (virtual node first):

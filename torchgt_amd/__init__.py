@@ -9,6 +9,8 @@ from .core_attention import (CoreAttention, SparseAttentionFunction, DenseAttent
 from .plan import GraphPlan, get_plan, clear_plan_cache, set_plan_cache_bytes
 from .multi_head_attention import MultiHeadAttention, LinearFunction, fused_linear
 from .encoder import FeedForwardNetwork, EncoderLayer, Graphormer, nll_loss
+from .gated_block import (GatedEncoderLayer, GatedFeedForwardNetwork, RMSNorm, add_rms_norm, add_rms_norm_8bit, gated_linear,
+                          gated_linear_8bit, linear_act, linear_act_8bit, quantize_rows)
 from .graph_bias import GraphAttnBias, floyd_warshall, gen_edge_input
 from .graph_level import GraphNodeFeature, Graphormer as GraphLevelGraphormer
 from .gt import GT, GraphLevelGT, MLPReadout
@@ -19,4 +21,6 @@ __all__ = ["CoreAttention", "SparseAttentionFunction", "DenseAttentionFunction",
            "GraphPlan", "get_plan", "clear_plan_cache", "set_plan_cache_bytes", "BlockAttentionFunction", "TileSet", "block_attention",
            "expand_tiles", "MultiHeadAttention", "LinearFunction", "fused_linear",
            "FeedForwardNetwork", "EncoderLayer", "Graphormer", "nll_loss", "GraphAttnBias", "floyd_warshall", "gen_edge_input",
-           "GraphNodeFeature", "GraphLevelGraphormer", "GT", "GraphLevelGT", "MLPReadout"]
+           "GraphNodeFeature", "GraphLevelGraphormer", "GT", "GraphLevelGT", "MLPReadout",
+           "RMSNorm", "GatedFeedForwardNetwork", "GatedEncoderLayer", "add_rms_norm", "add_rms_norm_8bit", "quantize_rows", "gated_linear",
+           "gated_linear_8bit", "linear_act", "linear_act_8bit"]

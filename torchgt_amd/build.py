@@ -14,7 +14,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ_DIR = os.path.join(CSRC, "build")
 LIB_PATH = os.path.join(HERE, "libtorchgt_hip.so")
-EXT_SRCS = [os.path.join(CSRC, f) for f in ("torch_binding.cpp", "torch_models.cpp", "torch_layered.cpp")]
+EXT_SRCS = [os.path.join(CSRC, f) for f in ("torch_binding.cpp", "torch_models.cpp", "torch_layered.cpp", "torch_gated.cpp")]
 EXT_PATH = os.path.join(HERE, "_torchgt_ext.so")
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -33,7 +33,8 @@ def sources():
 
 # sources compiled as several translation units (-D<macro>=k, k < parts), in parallel: their
 # kernels take minutes to compile in one piece
-SPLIT = {"sparse_attn.hip": ("TGT_SPARSE_PART", 4), "dense_attn.hip": ("TGT_DENSE_PART", 2), "dense_plane.hip": ("TGT_PLANE_PART", 3)}
+SPLIT = {"sparse_attn.hip": ("TGT_SPARSE_PART", 4), "dense_attn.hip": ("TGT_DENSE_PART", 2), "dense_plane.hip": ("TGT_PLANE_PART", 3),
+         "gated.hip": ("TGT_GATED_PART", 4)}
 
 
 def _jobs():

@@ -1,0 +1,389 @@
+// Products of matrices of any size in workgroup tiles, for the gated projections and the linears with an epilogue (gated.hip):
+//
+//   kForward   out[q, p] = sum_k Q[q, k] P[p, k]        x [N, K] against weights [F, K], both with k contiguous
+//   kInputGrad dx[q, p]  = sum_k Q[q, k] P[k, p]        du [N, F] against weights [F, K]: P's rows are the contraction
+//   kWeightGrad dW[q, p] = sum_k Q[k, q] P[k, p]        du [N, F] and x [N, K], nodes are the contraction
+//
+// q are the rows of what is written, p its columns.  P is the matrix instructions' A operand and Q their B: a lane then holds four
+// neighbouring columns of one row and writes them in one piece.  With two weights (gate and up) the forward's P alternates 16 rows of one with 16
+// of the other, so that a lane has both values of an element; the input gradient's contraction runs through the first weight's
+// rows and on through the second's.
+//
+// Matrix instructions: v_mfma_f32_16x16x32_bf16, for 8-bit operands v_mfma_scale_f32_16x16x128_f8f6f4 with block scales of one.
+//   A, B: lane l holds row l % 16, contraction indices of group l / 16;   C: lane l, register r: row 4 (l / 16) + r, column l % 16
+// float32 operands are cut into three bf16 parts that add up to them exactly, six of the nine products are formed (the other three are below
+// 2^-24 of the product).  An infinity times the other factor's zero part would be NaN: sums that come out NaN are formed again by
+// plain multiply-adds.
+#pragma once
+#include "common.h"
+
+namespace tgt {
+namespace gemm {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+struct b16 { uint16_t x; };      // bfloat16 in memory
+struct e4m3 { uint8_t x; };      // OCP e4m3 in memory
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(b16 v) { return __uint_as_float((uint32_t)v.x << 16); }
+__device__ __forceinline__ float to_float(e4m3 v) { return __builtin_amdgcn_cvt_f32_fp8((int)v.x, 0); }
+__device__ __forceinline__ void from_float(float& o, float v) { o = v; }
+__device__ __forceinline__ void from_float(b16& o, float v) { o.x = __builtin_bit_cast(uint16_t, static_cast<__bf16>(v)); }
+
+// The operand types: planes in LDS, contraction indices of a step and of a 16-byte piece of a plane
+template <typename T> struct Kind;
+template <> struct Kind<b16> { static constexpr int kPlanes = 1, kStep = 64, kPiece = 8, kRowBytes = 128; };
+template <> struct Kind<float> { static constexpr int kPlanes = 3, kStep = 32, kPiece = 8, kRowBytes = 64; };
+template <> struct Kind<e4m3> { static constexpr int kPlanes = 1, kStep = 128, kPiece = 16, kRowBytes = 128; };
+
+enum Form { kForward, kInputGrad, kWeightGrad };
+
+struct Args {
+    const void* P[2];          // the second one only with two weights
+    const void* Q;
+    int64_t p_ld, q_ld;        // elements from row to row
+    int64_t p_count, q_count;  // rows of each P (kForward), columns of P; rows of the result
+    int64_t K;                 // length of the contraction
+    int64_t K_first;           // kInputGrad: contraction indices of the first P (K if there is one)
+    int64_t K_each;            // contraction indices of one split, a multiple of the step
+    // epilogue
+    const void* bias[2];       // [p_count] or null
+    const void* residual;      // [q_count, p_count] or null
+    const void* dy;            // kForward with GRAD: the gradient of the result
+    const float* q_scale;      // 8-bit operands: one per row of Q and of each P
+    const float* p_scale[2];
+    void* out[2];              // kWeightGrad: out[1] has the rows from q_first on
+    int64_t out_ld;
+    int64_t q_first;
+    float* partial;            // kWeightGrad with more than one split: [splits][q_count][p_count]
+    int act;
+    unsigned p_tiles, q_tiles;
+};
+
+// ---- pieces of an operand on their way from memory to LDS --------------------------------------------------------------------------
+
+// Elements of a row that starts at any address: the compiler takes it from the type's alignment that wide loads may be misaligned
+template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Loose { u32x4 v; };
+
+template <typename T> struct Piece;      // a 16-byte piece of each plane, as it is in memory
+template <> struct Piece<b16> { u32x4 v; };
+template <> struct Piece<e4m3> { u32x4 v; };
+template <> struct Piece<float> { u32x4 v[2]; };
+
+template <typename T, bool ALIGNED> __device__ __forceinline__ u32x4 load16(const T* p) {
+    if constexpr (ALIGNED) return *reinterpret_cast<const u32x4*>(p);
+    else return reinterpret_cast<const Loose<T>*>(p)->v;
+}
+__device__ __forceinline__ u32x4 zero_unless(bool ok, u32x4 v) {
+    const uint32_t m = ok ? ~0u : 0u;
+    return u32x4{v.x & m, v.y & m, v.z & m, v.w & m};
+}
+
+// 16 bytes of a row from element `at` on, zero from `end` on.  `row` is readable over [0, end), end >= 1.  ALIGNED: row and end are multiples
+// of 16 bytes; the load is then unconditional (a branch around it would make every load wait for the one before).
+template <typename T, bool ALIGNED> __device__ __forceinline__ u32x4 part_of_row(const T* row, int64_t at, int64_t end, bool ok) {
+    constexpr int VE = 16 / (int)sizeof(T);
+    if constexpr (ALIGNED) {
+        const bool in = ok && at < end;
+        return zero_unless(in, load16<T, true>(row + (at < end ? at : 0)));
+    } else {
+        if (!ok || at >= end) return u32x4{0u, 0u, 0u, 0u};
+        if (at + VE <= end) return load16<T, false>(row + at);
+        union { T e[VE]; u32x4 v; } u;
+        u.v = u32x4{0u, 0u, 0u, 0u};
+        for (int i = 0; i < VE; ++i)
+            if (at + i < end) u.e[i] = row[at + i];
+        return u.v;
+    }
+}
+template <typename T, bool ALIGNED> __device__ __forceinline__ void fetch(Piece<T>& w, const T* row, int64_t at, int64_t end, bool ok) {
+    if constexpr (sizeof(T) == 4) {
+        w.v[0] = part_of_row<T, ALIGNED>(row, at, end, ok);
+        w.v[1] = part_of_row<T, ALIGNED>(row, at + 4, end, ok);
+    } else {
+        w.v = part_of_row<T, ALIGNED>(row, at, end, ok);
+    }
+}
+
+// float32 as three bf16 parts: each part is what is left with its low bits cut off, so a part never overflows and the three add up
+// exactly (24 bits are three times eight).  An infinity or a NaN is all in the first part.
+__device__ __forceinline__ void three_parts(float v, uint32_t& a, uint32_t& b, uint32_t& c) {
+    const uint32_t bits = __float_as_uint(v);
+    a = bits & 0xffff0000u;
+    const float r1 = (bits & 0x7f800000u) == 0x7f800000u ? 0.f : v - __uint_as_float(a);
+    b = __float_as_uint(r1) & 0xffff0000u;
+    c = __float_as_uint(r1 - __uint_as_float(b)) & 0xffff0000u;
+    // (a NaN whose payload is in the low half must stay one)
+    if ((bits & 0x7fffffffu) > 0x7f800000u) a |= 0x00400000u;
+}
+
+// Puts a piece at byte `at` of each plane
+template <typename T> __device__ __forceinline__ void put(char* lds, int plane_bytes, int at, const Piece<T>& w) {
+    if constexpr (sizeof(T) == 4) {
+        u32x4 p[3];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t a[2], b[2], c[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int e = 2 * i + j;
+                three_parts(__uint_as_float(w.v[e >> 2][e & 3]), a[j], b[j], c[j]);
+            }
+            p[0][i] = (a[0] >> 16) | a[1];
+            p[1][i] = (b[0] >> 16) | b[1];
+            p[2][i] = (c[0] >> 16) | c[1];
+        }
+#pragma unroll
+        for (int q = 0; q < 3; ++q) *reinterpret_cast<u32x4*>(lds + q * plane_bytes + at) = p[q];
+    } else {
+        *reinterpret_cast<u32x4*>(lds + at) = w.v;
+    }
+}
+
+// One operand's tile of COUNT rows (of the result's side).
+// Contraction contiguous (KC): LDS has rows of kRowBytes, their 16-byte pieces exchanged by a mask from the row, so that the 16 rows that an
+// operand read takes at one piece lie in different banks.
+// Contraction in rows (KM): LDS has [contraction][COUNT] as memory has, read back transposed (ds_read_b64_tr_b16); the 32-byte pieces of a row are
+// exchanged by a mask from its index, since the rows that one read takes are a multiple of all banks apart.
+template <typename T, bool KC, int COUNT, int THREADS, bool ALIGNED> struct Tile {
+    using K = Kind<T>;
+    static constexpr int kPlaneBytes = COUNT * K::kRowBytes, kBytes = kPlaneBytes * K::kPlanes;
+    static constexpr int kAcross = KC ? K::kRowBytes / 16 : COUNT / 8;      // pieces in a row of LDS
+    static constexpr int kRows = KC ? COUNT : K::kStep;
+    static constexpr int kEach = kRows * kAcross / THREADS;
+    static_assert(kRows * kAcross % THREADS == 0 && THREADS % kAcross == 0, "every thread has the same number of pieces, in rows a fixed step apart");
+    static_assert(KC || K::kPiece == 8, "transposed reads are for 16-bit planes");
+
+    Piece<T> w[kEach];
+    const T* row[KC ? kEach : 1];
+
+    static __device__ __forceinline__ int mask_of(int r) {
+        if (KC) return K::kRowBytes == 128 ? (r & 7) : ((r >> 2) & 3);
+        return (r & 3) | ((r >> 1) & 4);
+    }
+    static __device__ __forceinline__ int place(int r, int piece) {
+        if (KC) return r * K::kRowBytes + ((piece ^ mask_of(r)) << 4);
+        return r * (COUNT * 2) + ((((piece >> 1) ^ mask_of(r)) << 1 | (piece & 1)) << 4);
+    }
+
+    // KC: the rows' addresses.  TWO: 16 rows of the first matrix, 16 of the second, ...
+    template <bool TWO> __device__ __forceinline__ void begin(const void* const* base, int64_t ld, int64_t first, int64_t count) {
+        if constexpr (KC) {
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                const int r = threadIdx.x / kAcross + i * (THREADS / kAcross);
+                int64_t at = TWO ? first + (r >> 5) * 16 + (r & 15) : first + r;
+                const T* m = reinterpret_cast<const T*>(TWO && (r & 16) ? base[1] : base[0]);
+                at = at < count ? at : count - 1;      // (rows behind the last are computed and not written)
+                row[i] = m + at * ld;
+            }
+        }
+    }
+    __device__ __forceinline__ void fetch_contiguous(int64_t k0, int64_t K_end) {
+        const int64_t at = k0 + (threadIdx.x % kAcross) * K::kPiece;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) fetch<T, ALIGNED>(w[i], row[i], at, K_end, true);
+    }
+    // contraction rows k0 .. of a matrix (the second one's from K_first on), columns from first
+    template <bool TWO> __device__ __forceinline__ void fetch_rows(const void* const* base, int64_t ld, int64_t first, int64_t count, int64_t k0, int64_t K_end,
+                                                                   int64_t K_first) {
+        const int64_t col = first + (threadIdx.x % kAcross) * 8;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int64_t k = k0 + threadIdx.x / kAcross + i * (THREADS / kAcross);
+            const int64_t kk = k < K_end ? k : K_end - 1;
+            const T* m = reinterpret_cast<const T*>(base[0]) + kk * ld;
+            if (TWO && kk >= K_first) m = reinterpret_cast<const T*>(base[1]) + (kk - K_first) * ld;
+            fetch<T, ALIGNED>(w[i], m, col, count, k < K_end);
+        }
+    }
+    __device__ __forceinline__ void store(char* lds) const {
+        const int piece = threadIdx.x % kAcross;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int r = threadIdx.x / kAcross + i * (THREADS / kAcross);
+            put<T>(lds, kPlaneBytes, place(r, piece), w[i]);
+        }
+    }
+    // the 16 rows from 16 f on, contraction indices 32 s ..
+    static __device__ __forceinline__ bf16x8 operand(const char* lds, int plane, int f, int s) {
+        const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
+        const char* p = lds + plane * kPlaneBytes;
+        if constexpr (KC) {
+            return *reinterpret_cast<const bf16x8*>(p + place(16 * f + i, 4 * s + g));
+        } else {
+            typedef __attribute__((address_space(3))) i16x4* lds_i16x4;
+            const int k = 32 * s + 8 * g + (i >> 2);
+            const char* at = p + k * (COUNT * 2) + ((f ^ mask_of(k)) << 5) + (i & 3) * 8;
+            union { i16x4 h[2]; bf16x8 v; } u;
+            u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)(at));
+            u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)(at + 4 * (COUNT * 2)));      // (the mask leaves bit 2 out)
+            return u.v;
+        }
+    }
+    static __device__ __forceinline__ i32x8 operand8(const char* lds, int f) {
+        const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
+        union { u32x4 h[2]; i32x8 v; } u;
+        u.h[0] = *reinterpret_cast<const u32x4*>(lds + place(16 * f + i, g));
+        u.h[1] = *reinterpret_cast<const u32x4*>(lds + place(16 * f + i, g + 4));
+        return u.v;
+    }
+};
+
+}  // namespace gemm
+}  // namespace tgt
+
+// ---- the product of a workgroup's tile ---------------------------------------------------------------------------------------------
+namespace tgt {
+namespace gemm {
+
+// (the sum of one element once more, in plain multiply-adds: float32, where the parts' sum came out NaN)
+template <int FORM> __device__ __noinline__ float again(const Args& a, int which, int64_t q, int64_t p, int64_t k0, int64_t k1) {
+    const float* Q = reinterpret_cast<const float*>(a.Q);
+    const float* P = reinterpret_cast<const float*>(a.P[which]);
+    float s = 0.f;
+    for (int64_t k = k0; k < k1 && s == s; ++k) {
+        float y;
+        if (FORM == kForward) y = P[p * a.p_ld + k];
+        else if (FORM == kInputGrad) y = k < a.K_first ? P[k * a.p_ld + p] : reinterpret_cast<const float*>(a.P[1])[(k - a.K_first) * a.p_ld + p];
+        else y = P[k * a.p_ld + p];
+        s = __builtin_fmaf(FORM == kWeightGrad ? Q[k * a.q_ld + q] : Q[q * a.q_ld + k], y, s);
+    }
+    return s;
+}
+
+// Tile shape: COLS x ROWS of the result by WP x WQ waves
+template <int COLS, int ROWS, int WP_, int WQ_> struct Shape {
+    static constexpr int kCols = COLS, kRows = ROWS, WP = WP_, WQ = WQ_, kThreads = 64 * WP * WQ;
+    static constexpr int FP = COLS / WP / 16, FQ = ROWS / WQ / 16;      // 16 x 16 pieces of a wave
+};
+
+// acc[i][j]: columns 16 i .., rows 16 j .. of the wave's part of the tile.  lds: STAGES times the tiles' bytes.
+template <typename T, int FORM, bool TWO, bool ALIGNED, typename S, int STAGES>
+__device__ __forceinline__ void product(const Args& a, int64_t p0, int64_t q0, int64_t k0, int64_t k1, char* lds, f32x4 (&acc)[S::FP][S::FQ]) {
+    using K = Kind<T>;
+    constexpr bool kPC = FORM == kForward, kQC = FORM != kWeightGrad;
+    using PT = Tile<T, kPC, S::kCols, S::kThreads, ALIGNED>;
+    using QT = Tile<T, kQC, S::kRows, S::kThreads, ALIGNED>;
+    constexpr int kStage = PT::kBytes + QT::kBytes;
+    const int wave = threadIdx.x >> 6, wp = wave % S::WP, wq = wave / S::WP;
+    PT P;
+    QT Q;
+    P.template begin<TWO>(a.P, a.p_ld, p0, a.p_count);
+    const void* qs[2] = {a.Q, a.Q};
+    Q.template begin<false>(qs, a.q_ld, q0, a.q_count);
+#pragma unroll
+    for (int i = 0; i < S::FP; ++i)
+#pragma unroll
+        for (int j = 0; j < S::FQ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    auto load = [&](int64_t k) {
+        if constexpr (kPC) P.fetch_contiguous(k, k1);
+        else P.template fetch_rows<FORM == kInputGrad && TWO>(a.P, a.p_ld, p0, a.p_count, k, k1, a.K_first);
+        if constexpr (kQC) Q.fetch_contiguous(k, k1);
+        else Q.template fetch_rows<false>(qs, a.q_ld, q0, a.q_count, k, k1, k1);
+    };
+    auto multiply = [&](const char* at) {
+        const char *pl = at, *ql = at + PT::kBytes;
+        if constexpr (sizeof(T) == 1) {
+            i32x8 x[S::FP];
+#pragma unroll
+            for (int i = 0; i < S::FP; ++i) x[i] = PT::operand8(pl, wp * S::FP + i);
+#pragma unroll
+            for (int j = 0; j < S::FQ; ++j) {
+                const i32x8 y = QT::operand8(ql, wq * S::FQ + j);
+#pragma unroll
+                for (int i = 0; i < S::FP; ++i)
+                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x[i], y, acc[i][j], 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+            }
+        } else {
+#pragma unroll
+            for (int s = 0; s < K::kStep / 32; ++s) {
+                bf16x8 x[K::kPlanes][S::FP];
+#pragma unroll
+                for (int u = 0; u < K::kPlanes; ++u)
+#pragma unroll
+                    for (int i = 0; i < S::FP; ++i) x[u][i] = PT::operand(pl, u, wp * S::FP + i, s);
+#pragma unroll
+                for (int j = 0; j < S::FQ; ++j) {
+                    bf16x8 y[K::kPlanes];
+#pragma unroll
+                    for (int u = 0; u < K::kPlanes; ++u) y[u] = QT::operand(ql, u, wq * S::FQ + j, s);
+#pragma unroll
+                    for (int u = K::kPlanes - 1; u >= 0; --u)      // (the small products first)
+#pragma unroll
+                        for (int v = 0; v <= u; ++v)
+#pragma unroll
+                            for (int i = 0; i < S::FP; ++i)
+                                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[v][i], y[u - v], acc[i][j], 0, 0, 0);
+                }
+            }
+        }
+    };
+
+    load(k0);
+    if constexpr (STAGES == 2) {
+        P.store(lds);
+        Q.store(lds + PT::kBytes);
+        __syncthreads();
+        int cur = 0;
+        for (int64_t k = k0; k < k1; k += K::kStep) {
+            const bool more = k + K::kStep < k1;
+            if (more) load(k + K::kStep);
+            multiply(lds + cur * kStage);
+            cur ^= 1;      // (read last in the step before, and every wave has passed the barrier since)
+            if (more) {
+                P.store(lds + cur * kStage);
+                Q.store(lds + cur * kStage + PT::kBytes);
+            }
+            __syncthreads();
+        }
+    } else {
+        for (int64_t k = k0; k < k1; k += K::kStep) {
+            P.store(lds);
+            Q.store(lds + PT::kBytes);
+            __syncthreads();
+            if (k + K::kStep < k1) load(k + K::kStep);
+            multiply(lds);
+            __syncthreads();
+        }
+    }
+    if constexpr (sizeof(T) == 4) {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int i = 0; i < S::FP; ++i)
+#pragma unroll
+            for (int j = 0; j < S::FQ; ++j) {
+                const f32x4 c = acc[i][j];
+                if (__builtin_expect(c.x != c.x || c.y != c.y || c.z != c.z || c.w != c.w, 0)) {
+                    const bool two = FORM == kForward && TWO;
+                    const int f = wp * S::FP + i;
+                    const int64_t q = q0 + (wq * S::FQ + j) * 16 + (lane & 15), p = p0 + (two ? f >> 1 : f) * 16 + (lane >> 4) * 4;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (c[e] != c[e] && q < a.q_count && p + e < a.p_count) acc[i][j][e] = again<FORM>(a, two ? f & 1 : 0, q, p + e, k0, k1);
+                }
+            }
+    }
+}
+
+// Workgroup -> tile.  Consecutive workgroups go to the eight XCDs in turn, each with an L2 of its own: XCD x takes the tiles from x / 8 of
+// the way on, eight rows of tiles at a time, column by column, so that the tiles that run there together share both operands.
+__device__ __forceinline__ bool tile_of(const Args& a, unsigned b, unsigned& tp, unsigned& tq) {
+    const unsigned n = a.p_tiles * a.q_tiles, each = (n + 7) / 8, t = (b & 7) * each + (b >> 3);
+    if ((b >> 3) >= each || t >= n) return false;
+    constexpr unsigned kBand = 8;
+    const unsigned band = t / (kBand * a.p_tiles), rest = t - band * kBand * a.p_tiles;
+    const unsigned high = min(kBand, a.q_tiles - band * kBand);
+    tq = band * kBand + rest % high;
+    tp = rest / high;
+    return true;
+}
+
+}  // namespace gemm
+}  // namespace tgt

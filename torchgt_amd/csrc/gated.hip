@@ -1,0 +1,493 @@
+// The gated projections of a feed-forward block and linears with an epilogue, forward and backward, for matrices of any size:
+//
+//   gated   h = act(x Wg^T + bg) * (x Wu^T + bu)          both products, the activation and the product of the two in one kernel
+//   linear  y = act(x W^T + b) + residual
+//
+// No counterpart in the reference, whose feed-forward block has one projection and a GELU (models/graphormer_dist_node_level.py:27-39).
+//
+// Backward.  With g = x Wg^T + bg, u = x Wu^T + bu:  dg = dh u act'(g), du = dh act(g);  dx = dg Wg + du Wu;  dWg = dg^T x, dWu = du^T x; biases: column
+// sums.  g and u are not kept from the forward: a first kernel forms them again in float32 and writes dg and du side by side, [N, 2F] (rounded to
+// the tensors' type, since they are operands of the next two products; that costs as much as the rounding of any other activation).  Keeping
+// them would cost 4 F values of memory per node and their rounding would go into act'.  dx and dW are products of what it wrote.
+// dW over few output tiles is cut along the nodes, partial sums in float32 added in a fixed order.
+#include "block_gemm.h"
+#include <algorithm>
+
+namespace tgt {
+namespace {
+
+using namespace gemm;
+
+// act(u), and dh * act'(u).  SILU: u / (1 + exp(-u))
+template <bool EXACT> __device__ __forceinline__ float exp_of(float v) { return EXACT ? expf(v) : __expf(v); }
+template <bool EXACT> __device__ __forceinline__ float act_of(int act, float u) {
+    if (act == TGT_ACT_SILU) return u / (1.f + exp_of<EXACT>(-u));
+    if (act == TGT_ACT_GELU) return act_value<false>(u);
+    if (act == TGT_ACT_RELU) return act_value<true>(u);
+    return u;
+}
+template <bool EXACT> __device__ __forceinline__ float slope_of(int act, float u, float dh) {
+    if (act == TGT_ACT_SILU) {
+        const float s = 1.f / (1.f + exp_of<EXACT>(-u));
+        return dh * (s * (1.f + u * (1.f - s)));
+    }
+    if (act == TGT_ACT_GELU) return act_grad<false>(u, dh);
+    if (act == TGT_ACT_RELU) return act_grad<true>(u, dh);
+    return dh;
+}
+
+// Four neighbouring elements of a row, `n` of which exist; vec: the row is aligned for one access
+template <typename O> __device__ __forceinline__ void load4(const O* p, int n, bool vec, float (&f)[4]) {
+    O e[4] = {};
+    if (vec && n >= 4) {
+        if constexpr (sizeof(O) == 4) *reinterpret_cast<u32x4*>(e) = *reinterpret_cast<const u32x4*>(p);
+        else *reinterpret_cast<uint2*>(e) = *reinterpret_cast<const uint2*>(p);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < n) e[i] = p[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = to_float(e[i]);
+}
+template <typename O> __device__ __forceinline__ void store4(O* p, int n, bool vec, const float (&f)[4]) {
+    O e[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) from_float(e[i], f[i]);
+    if (vec && n >= 4) {
+        if constexpr (sizeof(O) == 4) *reinterpret_cast<u32x4*>(p) = *reinterpret_cast<const u32x4*>(e);
+        else *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(e);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < n) p[i] = e[i];
+    }
+}
+template <typename O> __device__ __forceinline__ bool fours(const void* p, int64_t ld) { return ((uintptr_t)p & (4 * sizeof(O) - 1)) == 0 && (ld & 3) == 0; }
+
+template <typename T, typename O, int FORM, bool TWO, bool GRAD, bool ALIGNED, typename S, int STAGES>
+__global__ __launch_bounds__(S::kThreads) void k_product(const Args a) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    constexpr bool kPair = FORM == kForward && TWO;
+    unsigned tp, tq;
+    if (!tile_of(a, blockIdx.x, tp, tq)) return;
+    const int64_t p0 = (int64_t)tp * (kPair ? S::kCols / 2 : S::kCols), q0 = (int64_t)tq * S::kRows;
+    const int64_t k0 = (int64_t)blockIdx.y * a.K_each, k1 = k0 + a.K_each < a.K ? k0 + a.K_each : a.K;
+    f32x4 acc[S::FP][S::FQ];
+    product<T, FORM, TWO, ALIGNED, S, STAGES>(a, p0, q0, k0, k1, lds, acc);
+
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wp = wave % S::WP, wq = wave / S::WP;
+    constexpr int kBy = kPair ? 2 : 1;      // pieces that one output piece takes
+    constexpr bool EXACT = sizeof(O) == 4;
+    const bool vec_out = fours<O>(a.out[0], a.out_ld) && (!a.out[1] || fours<O>(a.out[1], a.out_ld));
+#pragma unroll
+    for (int i = 0; i < S::FP; i += kBy) {
+        const int64_t p = p0 + (wp * S::FP + i) / kBy * 16 + (lane >> 4) * 4;
+        if (p >= a.p_count) continue;
+        const int n = a.p_count - p < 4 ? (int)(a.p_count - p) : 4;
+        float bias[kBy][4], scale[kBy][4];
+        if constexpr (FORM == kForward) {
+#pragma unroll
+            for (int w = 0; w < kBy; ++w) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { bias[w][e] = 0.f; scale[w][e] = 1.f; }
+                if (a.bias[w]) load4(reinterpret_cast<const O*>(a.bias[w]) + p, n, false, bias[w]);
+                if constexpr (sizeof(T) == 1) load4(a.p_scale[w] + p, n, false, scale[w]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < S::FQ; ++j) {
+            const int64_t q = q0 + (wq * S::FQ + j) * 16 + (lane & 15);
+            if (q >= a.q_count) continue;
+            if constexpr (FORM == kForward) {
+                float v[kBy][4];
+                const float qs = sizeof(T) == 1 ? a.q_scale[q] : 1.f;
+#pragma unroll
+                for (int w = 0; w < kBy; ++w)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float t = acc[i + w][j][e];
+                        if constexpr (sizeof(T) == 1) t *= qs * scale[w][e];
+                        v[w][e] = t + bias[w][e];
+                    }
+                float o[4];
+                if constexpr (GRAD) {
+                    float dy[4];
+                    load4(reinterpret_cast<const O*>(a.dy) + q * a.p_count + p, n, fours<O>(a.dy, a.p_count), dy);
+                    if constexpr (kPair) {
+                        float o2[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            o[e] = slope_of<EXACT>(a.act, v[0][e], dy[e] * v[1][e]);
+                            o2[e] = dy[e] * act_of<EXACT>(a.act, v[0][e]);
+                        }
+                        store4(reinterpret_cast<O*>(a.out[1]) + q * a.out_ld + p, n, vec_out, o2);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[e] = slope_of<EXACT>(a.act, v[0][e], dy[e]);
+                    }
+                } else {
+                    if constexpr (kPair) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[e] = act_of<EXACT>(a.act, v[0][e]) * v[1][e];
+                    } else {
+                        float r[4] = {0.f, 0.f, 0.f, 0.f};
+                        if (a.residual) load4(reinterpret_cast<const O*>(a.residual) + q * a.p_count + p, n, fours<O>(a.residual, a.p_count), r);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[e] = act_of<EXACT>(a.act, v[0][e]) + r[e];
+                    }
+                }
+                store4(reinterpret_cast<O*>(a.out[0]) + q * a.out_ld + p, n, vec_out, o);
+            } else {
+                const float o[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+                if (FORM == kWeightGrad && a.partial) {
+                    float* to = a.partial + ((int64_t)blockIdx.y * a.q_count + q) * a.p_count + p;
+                    store4(to, n, fours<float>(a.partial, a.p_count), o);
+                } else if (FORM == kWeightGrad && q >= a.q_first) {
+                    store4(reinterpret_cast<O*>(a.out[1]) + (q - a.q_first) * a.out_ld + p, n, vec_out, o);
+                } else {
+                    store4(reinterpret_cast<O*>(a.out[0]) + q * a.out_ld + p, n, vec_out, o);
+                }
+            }
+        }
+    }
+}
+
+#if TGT_GATED_PART == 0
+// Sums over the splits of a weight gradient, in their order.  Elements from q_first rows on go to the second output.
+template <typename O> __global__ __launch_bounds__(256) void k_add_splits(const float* __restrict__ partial, int splits, int64_t n, int64_t n_first, O* __restrict__ out0,
+                                                                          O* __restrict__ out1) {
+    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (e >= n) return;
+    float s = 0.f;
+    for (int w = 0; w < splits; ++w) s += partial[w * n + e];
+    O v;
+    from_float(v, s);
+    if (e < n_first) out0[e] = v;
+    else out1[e - n_first] = v;
+}
+
+// Column sums of a matrix of rows of M elements: workgroup (columns, share of the rows) -> partial[share][M]
+template <typename O> __global__ __launch_bounds__(256) void k_column_sums(const O* __restrict__ x, int64_t N, int64_t M, int64_t rows_each, float* __restrict__ partial) {
+    __shared__ float part[4][64];
+    const int c = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int64_t col = (int64_t)blockIdx.x * 64 + c, r0 = blockIdx.y * rows_each, r1 = r0 + rows_each < N ? r0 + rows_each : N;
+    float s = 0.f;
+    if (col < M)
+        for (int64_t r = r0 + w; r < r1; r += 4) s += to_float(x[r * M + col]);
+    part[w][c] = s;
+    __syncthreads();
+    if (w == 0 && col < M) partial[blockIdx.y * M + col] = (part[0][c] + part[1][c]) + (part[2][c] + part[3][c]);
+}
+
+__global__ __launch_bounds__(256) void k_zero(uint16_t* __restrict__ p, int64_t n) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = 0;
+}
+#endif
+
+using Square = Shape<128, 128, 2, 2>;
+
+template <typename T, typename O, int FORM, bool TWO, bool GRAD, bool ALIGNED, typename S, int STAGES>
+int launch(Args a, int splits, hipStream_t st) {
+    constexpr int kCols = FORM == kForward && TWO ? S::kCols / 2 : S::kCols;
+    a.p_tiles = (unsigned)((a.p_count + kCols - 1) / kCols);
+    a.q_tiles = (unsigned)((a.q_count + S::kRows - 1) / S::kRows);
+    const int64_t tiles = (int64_t)a.p_tiles * a.q_tiles;
+    if (tiles > (1ll << 30)) { set_error("torchgt: a product of more than 2^30 tiles"); return TGT_ERR_UNSUPPORTED; }
+    constexpr int kLds = STAGES * (S::kCols + S::kRows) * Kind<T>::kRowBytes * Kind<T>::kPlanes;
+    auto* kernel = k_product<T, O, FORM, TWO, GRAD, ALIGNED, S, STAGES>;
+    if (kLds > 65536) {
+        static std::atomic<uint64_t> done{0};
+        const int rc = allow_lds((const void*)kernel, kLds, done);
+        if (rc != TGT_OK) return rc;
+    }
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((tiles + 7) / 8 * 8), (unsigned)splits), dim3(S::kThreads), kLds, st, a);
+    TGT_HIP_CHECK(hipGetLastError());
+    return TGT_OK;
+}
+
+bool aligned16(const void* p, int64_t ld, int size) { return ((uintptr_t)p & 15) == 0 && ld * size % 16 == 0; }
+
+}  // namespace
+
+// One product in the form asked for; TWO: a.P[1] is given
+template <typename T, typename O> int product_forward(const Args& a, bool grad, hipStream_t st);
+template <typename T> int product_input_grad(const Args& a, hipStream_t st);
+template <typename T> int product_weight_grad(const Args& a, int splits, hipStream_t st);
+
+#if TGT_GATED_PART > 0
+template <typename T, typename O> int product_forward(const Args& a, bool grad, hipStream_t st) {
+    constexpr int kStages = sizeof(T) == 4 ? 1 : 2;
+    const bool two = a.P[1] != nullptr;
+    const bool al = aligned16(a.Q, a.q_ld, sizeof(T)) && aligned16(a.P[0], a.p_ld, sizeof(T)) && (!two || aligned16(a.P[1], a.p_ld, sizeof(T)));
+#define X(TWO, GRAD, AL) if (two == TWO && grad == GRAD && al == AL) return launch<T, O, kForward, TWO, GRAD, AL, Square, kStages>(a, 1, st)
+    X(false, false, true); X(true, false, true); X(false, false, false); X(true, false, false);
+    if constexpr (sizeof(T) > 1) { X(false, true, true); X(true, true, true); X(false, true, false); X(true, true, false); }
+#undef X
+    return TGT_ERR_INVALID_ARG;
+}
+#endif
+#if TGT_GATED_PART == 1 || TGT_GATED_PART == 2
+template <typename T> int product_input_grad(const Args& a, hipStream_t st) {
+    constexpr int kStages = sizeof(T) == 4 ? 1 : 2;
+    const bool two = a.P[1] != nullptr;
+    const bool al = aligned16(a.Q, a.q_ld, sizeof(T)) && aligned16(a.P[0], a.p_ld, sizeof(T)) && (!two || aligned16(a.P[1], a.p_ld, sizeof(T)));
+#define X(TWO, AL) if (two == TWO && al == AL) return launch<T, T, kInputGrad, TWO, false, AL, Square, kStages>(a, 1, st)
+    X(false, true); X(true, true); X(false, false); X(true, false);
+#undef X
+    return TGT_ERR_INVALID_ARG;
+}
+template <typename T> int product_weight_grad(const Args& a, int splits, hipStream_t st) {
+    constexpr int kStages = sizeof(T) == 4 ? 1 : 2;
+    if (aligned16(a.Q, a.q_ld, sizeof(T)) && aligned16(a.P[0], a.p_ld, sizeof(T))) return launch<T, T, kWeightGrad, false, false, true, Square, kStages>(a, splits, st);
+    return launch<T, T, kWeightGrad, false, false, false, Square, kStages>(a, splits, st);
+}
+#endif
+#if TGT_GATED_PART == 1
+template int product_forward<b16, b16>(const Args&, bool, hipStream_t);
+template int product_input_grad<b16>(const Args&, hipStream_t);
+template int product_weight_grad<b16>(const Args&, int, hipStream_t);
+#elif TGT_GATED_PART == 2
+template int product_forward<float, float>(const Args&, bool, hipStream_t);
+template int product_input_grad<float>(const Args&, hipStream_t);
+template int product_weight_grad<float>(const Args&, int, hipStream_t);
+#elif TGT_GATED_PART == 3
+template int product_forward<e4m3, b16>(const Args&, bool, hipStream_t);
+template int product_forward<e4m3, float>(const Args&, bool, hipStream_t);
+#else
+
+namespace {
+
+// What the entry points share: n weights [F, K] (two: gate and up)
+struct Call {
+    const char* who;
+    const void *x, *W[2], *b[2];
+    int n;
+    int64_t N;
+    int K, F, dtype, act;
+};
+
+int check_call(const Call& c, int64_t most_rows = 0x7fffffff) {
+    if (c.N < 0 || c.K < 1 || c.F < 1 || (c.dtype != TGT_DTYPE_F32 && c.dtype != TGT_DTYPE_BF16)) {
+        set_error("%s: bad size or dtype", c.who);
+        return TGT_ERR_INVALID_ARG;
+    }
+    if (c.N > most_rows || c.F > (1 << 24) || c.K > (1 << 24)) {
+        set_error("%s: %lld rows of %d and %d features: at most 2^31 - 1 rows and 2^24 features", c.who, (long long)c.N, c.K, c.F);
+        return TGT_ERR_UNSUPPORTED;
+    }
+    if (c.act != TGT_ACT_NONE && c.act != TGT_ACT_GELU && c.act != TGT_ACT_RELU && c.act != TGT_ACT_SILU) {
+        set_error("%s: unknown activation %d", c.who, c.act);
+        return TGT_ERR_INVALID_ARG;
+    }
+    if (c.N > 0 && (!c.x || !c.W[0] || (c.n == 2 && !c.W[1]))) {
+        set_error("%s: null pointer", c.who);
+        return TGT_ERR_INVALID_ARG;
+    }
+    return TGT_OK;
+}
+
+Args forward_args(const Call& c) {
+    Args a{};
+    a.P[0] = c.W[0]; a.P[1] = c.n == 2 ? c.W[1] : nullptr;
+    a.Q = c.x;
+    a.p_ld = a.q_ld = c.K;
+    a.p_count = c.F; a.q_count = c.N;
+    a.K = a.K_first = a.K_each = c.K;
+    a.bias[0] = c.b[0]; a.bias[1] = c.n == 2 ? c.b[1] : nullptr;
+    a.out_ld = c.F;
+    a.act = c.act;
+    return a;
+}
+
+int forward(const Call& c, const void* residual, void* out, hipStream_t st) {
+    int rc = check_call(c);
+    if (rc != TGT_OK || c.N == 0) return rc;
+    if (!out) { set_error("%s: null pointer", c.who); return TGT_ERR_INVALID_ARG; }
+    Args a = forward_args(c);
+    a.residual = residual;
+    a.out[0] = out;
+    KernelTimer t(KS_LINEAR_FWD, st);
+    return c.dtype == TGT_DTYPE_F32 ? product_forward<float, float>(a, false, st) : product_forward<b16, b16>(a, false, st);
+}
+
+int forward_8bit(const Call& c, const float* x_scales, const float* s0, const float* s1, const void* residual, void* out, hipStream_t st) {
+    int rc = check_call(c);
+    if (rc != TGT_OK) return rc;
+    if (c.K % 16) {
+        set_error("%s: %d features: operands in 8 bits need a multiple of 16", c.who, c.K);
+        return TGT_ERR_UNSUPPORTED;
+    }
+    if (c.N == 0) return TGT_OK;
+    if (!out || !x_scales || !s0 || (c.n == 2 && !s1)) { set_error("%s: null pointer", c.who); return TGT_ERR_INVALID_ARG; }
+    Args a = forward_args(c);
+    a.q_scale = x_scales;
+    a.p_scale[0] = s0; a.p_scale[1] = s1;
+    a.residual = residual;
+    a.out[0] = out;
+    KernelTimer t(KS_LINEAR_FWD, st);
+    return c.dtype == TGT_DTYPE_F32 ? product_forward<e4m3, float>(a, false, st) : product_forward<e4m3, b16>(a, false, st);
+}
+
+// How the backward lays out its workspace, and how it cuts the nodes
+struct Plan {
+    int64_t du_bytes, bytes, K_each, rows_each;
+    int splits, shares;
+};
+int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
+Plan plan_of(int n, int64_t N, int K, int F, int dtype, int act) {
+    Plan p{};
+    const int64_t size = dtype == TGT_DTYPE_F32 ? 4 : 2, cols = (int64_t)n * F;
+    const int step = dtype == TGT_DTYPE_F32 ? Kind<float>::kStep : Kind<b16>::kStep;
+    p.du_bytes = n == 2 || act != TGT_ACT_NONE ? up16(N * cols * size) : 0;      // (without an activation dy is the operand itself)
+    // two workgroups per CU: fewer tiles than that are cut along the nodes, in pieces of eight steps at least
+    const int64_t tiles = ((cols + 127) / 128) * (((int64_t)K + 127) / 128);
+    const int64_t want = std::max<int64_t>(1, std::min<int64_t>((512 + tiles - 1) / tiles, (N + 8 * step - 1) / (8 * step)));
+    p.K_each = ((N + want - 1) / std::max<int64_t>(1, want) + step - 1) / step * step;
+    p.splits = N > 0 ? (int)((N + p.K_each - 1) / p.K_each) : 1;
+    p.shares = (int)std::max<int64_t>(1, std::min<int64_t>(256, (N + 127) / 128));
+    p.rows_each = (N + p.shares - 1) / p.shares;
+    p.bytes = p.du_bytes + (p.splits > 1 ? up16((int64_t)p.splits * cols * K * 4) : 0) + up16((int64_t)p.shares * cols * 4);
+    return p;
+}
+
+int backward(const Call& c, const void* dy, void* dx, void* const* dW, void* const* db, void* workspace, int64_t workspace_bytes, hipStream_t st) {
+    int rc = check_call(c);
+    if (rc != TGT_OK) return rc;
+    const bool f32 = c.dtype == TGT_DTYPE_F32;
+    const int64_t size = f32 ? 4 : 2, cols = (int64_t)c.n * c.F;
+    const bool want_w = dW && dW[0], want_b = db && (db[0] || (c.n == 2 && db[1]));
+    if (want_w && c.n == 2 && !dW[1]) { set_error("%s: both weights' gradients or none", c.who); return TGT_ERR_INVALID_ARG; }
+    if (c.N == 0) {      // nothing to add up
+        for (int w = 0; w < c.n; ++w) {
+            const int64_t m = (int64_t)c.F * c.K * (size / 2), v = c.F * (size / 2);
+            if (want_w) hipLaunchKernelGGL(k_zero, dim3((unsigned)std::min<int64_t>((m + 255) / 256, 4096)), dim3(256), 0, st, (uint16_t*)dW[w], m);
+            if (want_b && db[w]) hipLaunchKernelGGL(k_zero, dim3((unsigned)std::min<int64_t>((v + 255) / 256, 4096)), dim3(256), 0, st, (uint16_t*)db[w], v);
+        }
+        TGT_HIP_CHECK(hipGetLastError());
+        return TGT_OK;
+    }
+    if (!dy) { set_error("%s: null pointer", c.who); return TGT_ERR_INVALID_ARG; }
+    const Plan p = plan_of(c.n, c.N, c.K, c.F, c.dtype, c.act);
+    if (!workspace || workspace_bytes < p.bytes || ((uintptr_t)workspace & 15)) {
+        set_error("%s: workspace of %lld bytes (16-byte aligned) needed, got %lld", c.who, (long long)p.bytes, (long long)workspace_bytes);
+        return TGT_ERR_WORKSPACE;
+    }
+    char* ws = (char*)workspace;
+    const void* du = dy;
+    if (p.du_bytes) {
+        Args a = forward_args(c);
+        a.dy = dy;
+        a.out[0] = ws;
+        a.out[1] = c.n == 2 ? ws + c.F * size : nullptr;
+        a.out_ld = cols;
+        KernelTimer t(KS_LINEAR_FWD, st);
+        rc = f32 ? product_forward<float, float>(a, true, st) : product_forward<b16, b16>(a, true, st);
+        if (rc != TGT_OK) return rc;
+        du = ws;
+    }
+    if (dx) {
+        Args a{};
+        a.P[0] = c.W[0]; a.P[1] = c.n == 2 ? c.W[1] : nullptr;
+        a.Q = du;
+        a.p_ld = c.K; a.q_ld = cols;
+        a.p_count = c.K; a.q_count = c.N;
+        a.K = a.K_each = cols; a.K_first = c.F;
+        a.out[0] = dx;
+        a.out_ld = c.K;
+        KernelTimer t(KS_LINEAR_DX, st);
+        rc = f32 ? product_input_grad<float>(a, st) : product_input_grad<b16>(a, st);
+        if (rc != TGT_OK) return rc;
+    }
+    char* after = ws + p.du_bytes;
+    if (want_w) {
+        Args a{};
+        a.P[0] = c.x;
+        a.Q = du;
+        a.p_ld = c.K; a.q_ld = cols;
+        a.p_count = c.K; a.q_count = cols;
+        a.K = a.K_first = c.N; a.K_each = p.K_each;
+        a.out[0] = dW[0]; a.out[1] = c.n == 2 ? dW[1] : nullptr;
+        a.q_first = c.F;
+        a.out_ld = c.K;
+        a.partial = p.splits > 1 ? (float*)after : nullptr;
+        KernelTimer t(KS_LINEAR_DW, st);
+        rc = f32 ? product_weight_grad<float>(a, p.splits, st) : product_weight_grad<b16>(a, p.splits, st);
+        if (rc != TGT_OK) return rc;
+        if (p.splits > 1) {
+            const int64_t n = cols * c.K, first = (int64_t)c.F * c.K;
+            const dim3 grid((unsigned)((n + 255) / 256));
+            if (f32) hipLaunchKernelGGL((k_add_splits<float>), grid, dim3(256), 0, st, a.partial, p.splits, n, first, (float*)dW[0], (float*)a.out[1]);
+            else hipLaunchKernelGGL((k_add_splits<b16>), grid, dim3(256), 0, st, a.partial, p.splits, n, first, (b16*)dW[0], (b16*)a.out[1]);
+            TGT_HIP_CHECK(hipGetLastError());
+        }
+    }
+    if (want_b) {
+        float* partial = (float*)(ws + p.bytes - up16((int64_t)p.shares * cols * 4));
+        const dim3 grid((unsigned)((cols + 63) / 64), (unsigned)p.shares);
+        if (f32) hipLaunchKernelGGL((k_column_sums<float>), grid, dim3(256), 0, st, (const float*)du, c.N, cols, p.rows_each, partial);
+        else hipLaunchKernelGGL((k_column_sums<b16>), grid, dim3(256), 0, st, (const b16*)du, c.N, cols, p.rows_each, partial);
+        TGT_HIP_CHECK(hipGetLastError());
+        tgt_reduce_desc r{};
+        r.partial = partial; r.workers = p.shares; r.n = (int)cols; r.n_out = c.n;
+        r.out[0] = db[0]; r.begin[0] = 0;
+        if (c.n == 2) { r.out[1] = db[1]; r.begin[1] = c.F; }
+        return reduce_partials(&r, 1, c.dtype, st);
+    }
+    return TGT_OK;
+}
+
+int64_t workspace_bytes_of(int n, int64_t N, int K, int F, int dtype, int act) {
+    if (N < 0 || K < 1 || F < 1 || (dtype != TGT_DTYPE_F32 && dtype != TGT_DTYPE_BF16)) return -1;
+    return N == 0 ? 0 : plan_of(n, N, K, F, dtype, act).bytes;
+}
+
+}  // namespace
+#endif
+}  // namespace tgt
+
+#if TGT_GATED_PART == 0
+extern "C" {
+
+int tgt_gated_linear_fwd(const void* d_x, const void* d_Wg, const void* d_Wu, const void* d_bg, const void* d_bu, int64_t N, int in_features, int out_features,
+                         int dtype, int act, void* d_h, void* stream) {
+    const tgt::Call c{"tgt_gated_linear_fwd", d_x, {d_Wg, d_Wu}, {d_bg, d_bu}, 2, N, in_features, out_features, dtype, act};
+    return tgt::forward(c, nullptr, d_h, (hipStream_t)stream);
+}
+int tgt_gated_linear_8bit_fwd(const void* d_x, const float* d_x_scales, const void* d_Wg, const float* d_Wg_scales, const void* d_Wu, const float* d_Wu_scales,
+                              const void* d_bg, const void* d_bu, int64_t N, int in_features, int out_features, int dtype, int act, void* d_h, void* stream) {
+    const tgt::Call c{"tgt_gated_linear_8bit_fwd", d_x, {d_Wg, d_Wu}, {d_bg, d_bu}, 2, N, in_features, out_features, dtype, act};
+    return tgt::forward_8bit(c, d_x_scales, d_Wg_scales, d_Wu_scales, nullptr, d_h, (hipStream_t)stream);
+}
+int64_t tgt_gated_linear_bwd_workspace_bytes(int64_t N, int in_features, int out_features, int dtype) {
+    return tgt::workspace_bytes_of(2, N, in_features, out_features, dtype, TGT_ACT_SILU);
+}
+int tgt_gated_linear_bwd(const void* d_x, const void* d_Wg, const void* d_Wu, const void* d_bg, const void* d_bu, const void* d_dh, int64_t N, int in_features,
+                         int out_features, int dtype, int act, void* d_dx, void* const* d_dW, void* const* d_db, void* d_workspace, int64_t workspace_bytes,
+                         void* stream) {
+    const tgt::Call c{"tgt_gated_linear_bwd", d_x, {d_Wg, d_Wu}, {d_bg, d_bu}, 2, N, in_features, out_features, dtype, act};
+    return tgt::backward(c, d_dh, d_dx, d_dW, d_db, d_workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+int tgt_linear_epilogue_fwd(const void* d_x, const void* d_W, const void* d_b, const void* d_residual, int64_t N, int in_features, int out_features, int dtype,
+                            int act, void* d_y, void* stream) {
+    const tgt::Call c{"tgt_linear_epilogue_fwd", d_x, {d_W, nullptr}, {d_b, nullptr}, 1, N, in_features, out_features, dtype, act};
+    return tgt::forward(c, d_residual, d_y, (hipStream_t)stream);
+}
+int tgt_linear_epilogue_8bit_fwd(const void* d_x, const float* d_x_scales, const void* d_W, const float* d_W_scales, const void* d_b, const void* d_residual,
+                                 int64_t N, int in_features, int out_features, int dtype, int act, void* d_y, void* stream) {
+    const tgt::Call c{"tgt_linear_epilogue_8bit_fwd", d_x, {d_W, nullptr}, {d_b, nullptr}, 1, N, in_features, out_features, dtype, act};
+    return tgt::forward_8bit(c, d_x_scales, d_W_scales, nullptr, d_residual, d_y, (hipStream_t)stream);
+}
+int64_t tgt_linear_epilogue_bwd_workspace_bytes(int64_t N, int in_features, int out_features, int dtype, int act) {
+    return tgt::workspace_bytes_of(1, N, in_features, out_features, dtype, act);
+}
+int tgt_linear_epilogue_bwd(const void* d_x, const void* d_W, const void* d_b, const void* d_dy, int64_t N, int in_features, int out_features, int dtype, int act,
+                            void* d_dx, void* d_dW, void* d_db, void* d_workspace, int64_t workspace_bytes, void* stream) {
+    const tgt::Call c{"tgt_linear_epilogue_bwd", d_x, {d_W, nullptr}, {d_b, nullptr}, 1, N, in_features, out_features, dtype, act};
+    void *dW[2] = {d_dW, nullptr}, *db[2] = {d_db, nullptr};
+    return tgt::backward(c, d_dy, d_dx, dW, db, d_workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+}  // extern "C"
+#endif

@@ -19,6 +19,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import _ext, _lib
+from .gated_block import GatedEncoderLayer, RMSNorm, add_rms_norm
 from .module_tree import DROPOUT, OneWalk, all_plain, at_work, kind, model_parameters
 from .multi_head_attention import MultiHeadAttention, attention_modules, fused_linear, plain_attention, _DT
 from .plan import GraphPlan, get_plan
@@ -159,18 +160,24 @@ def layer_modules(count, layer):
 
 class Graphormer(OneWalk):
     """Graphormer for node-level tasks, global token at index 0
-    (models/graphormer_dist_node_level.py:316-392)."""
+    (models/graphormer_dist_node_level.py:316-392).  ``gated=True``: its layers are ``GatedEncoderLayer`` and its last norm is
+    an ``RMSNorm``; it runs layer by layer."""
+
+    gated = False
 
     def __init__(self, n_layers, num_heads, input_dim, hidden_dim, output_dim, attn_bias_dim, dropout_rate,
-                 input_dropout_rate, attention_dropout_rate, ffn_dim, num_global_node):
+                 input_dropout_rate, attention_dropout_rate, ffn_dim, num_global_node, gated=False):
         super().__init__()
+        if gated:
+            self.gated = True
         self.num_heads = num_heads
         self.node_encoder = nn.Linear(input_dim, hidden_dim)
         self.input_dropout = nn.Dropout(input_dropout_rate)
-        self.layers = nn.ModuleList([EncoderLayer(hidden_dim, ffn_dim, dropout_rate, attention_dropout_rate, num_heads,
-                                                  attn_bias_dim) for _ in range(n_layers)])
+        layer = GatedEncoderLayer if gated else EncoderLayer
+        self.layers = nn.ModuleList([layer(hidden_dim, ffn_dim, dropout_rate, attention_dropout_rate, num_heads,
+                                           attn_bias_dim) for _ in range(n_layers)])
         self.n_layers = n_layers
-        self.final_ln = nn.LayerNorm(hidden_dim)
+        self.final_ln = RMSNorm(hidden_dim) if gated else nn.LayerNorm(hidden_dim)
         self.downstream_out_proj = nn.Linear(hidden_dim, output_dim)
         self.hidden_dim = hidden_dim
         self.num_global_node = num_global_node
@@ -185,7 +192,7 @@ class Graphormer(OneWalk):
         attention without a bias, no dropout at work, every linear with its bias, one dtype, one global token (the rows that
         come back are 1 .. of the sequence, :391, whatever the number of tokens: the operators return the nodes' rows) -
         else None."""
-        if not self.one_operator or self.num_global_node != 1 or attn_type != "sparse" or attn_bias is not None or perturb is not None or edge_index is None:
+        if not self.one_operator or self.gated or self.num_global_node != 1 or attn_type != "sparse" or attn_bias is not None or perturb is not None or edge_index is None:
             return None
         if x.dim() != 2 or x.shape[0] == 0 or not x.is_cuda or x.dtype not in _DT or autocast_to_float32(x):
             return None
@@ -250,7 +257,10 @@ class Graphormer(OneWalk):
             output, pending = enc_layer(output, attn_bias=graph_attn_bias, edge_index=edge_index, attn_type=attn_type,
                                         residual=pending, defer_residual=True)
         fl = self.final_ln
-        _, output = _ext.op("add_layer_norm")(output, pending, fl.weight, fl.bias, float(fl.eps))
+        if self.gated:
+            _, output = add_rms_norm(output, pending, fl.weight, fl.eps)
+        else:
+            _, output = _ext.op("add_layer_norm")(output, pending, fl.weight, fl.bias, float(fl.eps))
         # rows 1.. of graph 0 (:391 `output[0, 1:, :]`); through a view, so that autograd pads the gradient once, not twice
         (output,) = fused_linear(output.reshape(-1, self.hidden_dim)[1:output.shape[1]], self.downstream_out_proj)
         return F.log_softmax(output, dim=1)
