@@ -666,3 +666,71 @@ def test_refusals(cuda):
         dual = fwAD.make_dual(x, torch.ones_like(x))
         with pytest.raises((RuntimeError, NotImplementedError)):
             T.gated_linear(dual, wg, wu)
+
+
+# ---- sizes that go to other variants -----------------------------------------------------------------------------------------------------------------
+
+def sampled(rows, cols, g):
+    return torch.randint(rows, (40,), generator=g), torch.randint(cols, (40,), generator=g)
+
+
+@pytest.mark.parametrize("shape", [(16384, 256, 2048), (13000, 320, 2176), (12929, 328, 2184), (5000, 1288, 1480), (3001, 2048, 4352)])
+def test_large_products_in_bf16(cuda, shape):
+    """Whole tiles of 256 and what is left of them, against a float32 product of the same operands on the GPU (exact products, sums off by sums(n) of the magnitudes
+    on either side), and element by element in 64 bits at sampled places with the last rows and columns among them."""
+    N, K, F = shape
+    x, wg, wu, bg, bu, dh = gated_case(N, K, F, BF16, "silu", True)
+    outs = run_gated(x, wg, wu, bg, bu, dh, "silu")
+    y = run_linear(x, wg, bg, dh, dh, "gelu")
+    yn = run_linear(x, wg, bg, dh, dh, None)
+    g = torch.Generator().manual_seed(1)
+    rows = torch.cat([torch.tensor([0, N - 1, N - 2, (N - 1) // 256 * 256]), torch.randint(N, (28,), generator=g)])
+    X, DH = d(x[rows]), d(dh[rows])
+    check_gated(x[rows], wg, wu, bg, bu, None, "silu", {"h": outs["h"][rows]})
+    check_linear(x[rows], wg, bg, dh[rows], None, "gelu", {"y": y["y"][rows]})
+    check_linear(x[rows], wg, bg, dh[rows], None, None, {"y": yn["y"][rows]})
+    WG, WU, BG, BU = d(wg), d(wu), d(bg), d(bu)
+    p, q = Mapped(X, WG, BG), Mapped(X, WU, BU)
+    s, a = slope64("silu", p.v), act64("silu", p.v)
+    dg, du = DH * q.v * s, DH * a
+    edg = stored(dg, DH.abs() * (q.v.abs() * (0.8 * p.e + fine(BF16) * (1 + p.v.abs())) + (s.abs() + 0.8 * p.e) * q.e) + 2.0 ** -22 * dg.abs(), BF16)
+    edu = stored(du, DH.abs() * (1.13 * p.e + fine(BF16) * (p.v.abs() + p.e)) + 2.0 ** -22 * du.abs(), BF16)
+    dx = Mapped(torch.cat([dg, du], 1), torch.cat([WG, WU]).T, ea=torch.cat([edg, edu], 1))
+    near(outs["x"][rows], dx.v, stored(dx.v, dx.e, BF16), "dx")
+    dxn = Mapped(DH, WG.T)
+    near(yn["x"][rows], dxn.v, stored(dxn.v, dxn.e, BF16), "dx of the linear")
+    # weight gradients: sampled rows f, the last among them
+    fs = torch.cat([torch.tensor([0, F - 1, F - 2, (F - 1) // 256 * 256]), torch.randint(F, (12,), generator=g)])
+    X, DH = d(x), d(dh[:, fs])
+    p, q = Mapped(X, WG[fs], BG[fs]), Mapped(X, WU[fs], BU[fs])
+    s, a = slope64("silu", p.v), act64("silu", p.v)
+    dg, du = DH * q.v * s, DH * a
+    edg = stored(dg, DH.abs() * (q.v.abs() * (0.8 * p.e + fine(BF16) * (1 + p.v.abs())) + (s.abs() + 0.8 * p.e) * q.e) + 2.0 ** -22 * dg.abs(), BF16)
+    edu = stored(du, DH.abs() * (1.13 * p.e + fine(BF16) * (p.v.abs() + p.e)) + 2.0 ** -22 * du.abs(), BF16)
+    for got, v, e in ((outs["wg"], dg, edg), (outs["wu"], du, edu), (yn["w"], DH, torch.zeros_like(DH))):
+        dw = Mapped(v.T, X.T, ea=e.T)
+        near(got[fs], dw.v, stored(dw.v, dw.e, BF16), "dW")
+    for got, v, e in ((outs["bg"], dg, edg), (outs["bu"], du, edu), (yn["b"], DH, torch.zeros_like(DH))):
+        near(got[fs], v.sum(0), stored(v.sum(0), e.sum(0) + sums(N) * v.abs().sum(0), BF16), "db")
+    again = run_gated(x, wg, wu, bg, bu, dh, "silu")
+    assert all(torch.equal(outs[k], again[k]) for k in outs)
+
+
+@pytest.mark.parametrize("shape", [(8200, 256, 2048), (5001, 1040, 2100), (2050, 2048, 6144)])
+@pytest.mark.parametrize("out", [F32, BF16])
+def test_large_products_in_8_bits(cuda, shape, out):
+    N, K, F = shape
+    g = torch.Generator().manual_seed(K)
+    x, xs = T.quantize_rows(rand(g, N, K, dt=BF16) * 3)
+    (wg, gs), (wu, us) = (T.quantize_rows(rand(g, F, K, dt=BF16, scale=1.2 / math.sqrt(K))) for _ in range(2))
+    bg, r = rand(g, F, dt=out, scale=0.3), rand(g, N, F, dt=out)
+    h = T.gated_linear_8bit(x, xs, wg, gs, wu, us, bg, bg, dtype=out)
+    y = T.linear_act_8bit(x, xs, wg, gs, bg, "relu", r, dtype=out)
+    rows = torch.tensor([0, 1, 255, 256, N // 2, N - 2, N - 1])
+    X = x[rows.cuda()].float().double().cpu() * d(xs[rows])[:, None]
+    WG, WU = (c.float().double().cpu() * d(s)[:, None] for c, s in ((wg, gs), (wu, us)))
+    p, q = Mapped(X, WG, d(bg), eight=True), Mapped(X, WU, d(bg), eight=True)
+    a = act64("silu", p.v)
+    want = a * q.v
+    near(h[rows], want, stored(want, (1.13 * p.e + fine(out) * (p.v.abs() + p.e)) * (q.v.abs() + q.e) + a.abs() * q.e + 2.0 ** -23 * want.abs(), out), "h")
+    check_linear(X, WG, d(bg), d(r[rows]), None, "relu", {"y": y[rows]}, eight=True)

@@ -9,7 +9,8 @@
 // of the other, so that a lane has both values of an element; the input gradient's contraction runs through the first weight's
 // rows and on through the second's.
 //
-// Matrix instructions: v_mfma_f32_16x16x32_bf16, for 8-bit operands v_mfma_scale_f32_16x16x128_f8f6f4 with block scales of one.
+// Matrix instructions: v_mfma_f32_16x16x32_bf16, for 8-bit operands v_mfma_f32_16x16x128_f8f6f4 (the builtin with
+// scales of zero is the instruction without block scales).
 //   A, B: lane l holds row l % 16, contraction indices of group l / 16;   C: lane l, register r: row 4 (l / 16) + r, column l % 16
 // float32 operands are cut into three bf16 parts that add up to them exactly, six of the nine products are formed (the other three are below
 // 2^-24 of the product).  An infinity times the other factor's zero part would be NaN: sums that come out NaN are formed again by
@@ -261,6 +262,9 @@ template <int FORM> __device__ __noinline__ float again(const Args& a, int which
 template <int COLS, int ROWS, int WP_, int WQ_> struct Shape {
     static constexpr int kCols = COLS, kRows = ROWS, WP = WP_, WQ = WQ_, kThreads = 64 * WP * WQ;
     static constexpr int FP = COLS / WP / 16, FQ = ROWS / WQ / 16;      // 16 x 16 pieces of a wave
+    // which 16 columns / rows of the tile a wave's piece is
+    static __device__ __forceinline__ int p_piece(int wave, int i) { return wave % WP * FP + i; }
+    static __device__ __forceinline__ int q_piece(int wave, int j) { return wave / WP * FQ + j; }
 };
 
 // acc[i][j]: columns 16 i .., rows 16 j .. of the wave's part of the tile.  lds: STAGES times the tiles' bytes.
@@ -299,7 +303,7 @@ __device__ __forceinline__ void product(const Args& a, int64_t p0, int64_t q0, i
                 const i32x8 y = QT::operand8(ql, wq * S::FQ + j);
 #pragma unroll
                 for (int i = 0; i < S::FP; ++i)
-                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x[i], y, acc[i][j], 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x[i], y, acc[i][j], 0, 0, 0, 0, 0, 0);
             }
         } else {
 #pragma unroll
@@ -384,6 +388,223 @@ __device__ __forceinline__ bool tile_of(const Args& a, unsigned b, unsigned& tp,
     tp = rest / high;
     return true;
 }
+
+// ---- large products of 16- and 8-bit operands ----------------------------------------------------------------------------------------
+//
+// Eight waves, 128 PH x 256 of the result, one workgroup to a CU that goes from tile to tile.  Operands go from memory straight to LDS
+// (global_load_lds, 16 bytes a lane), two steps deep; each half of an operand's tile (16 KB) is asked for again as soon as the
+// whole workgroup has read it, nearly two steps ahead.  Waves 0-3 and 4-7 - on each SIMD one of either - run one barrier apart: while one half of
+// them multiplies, the other reads its next operands from LDS.  A step has PH x 2 turns of 16 matrix instructions; a wave's counter of
+// outstanding loads is waited down to what was asked for after the halves that the next turn reads, so loads stay in flight over every barrier.
+//
+// A contraction that ends inside a step reads zeros for the rest: lanes past its end are pointed at 16 bytes of them.
+
+static __device__ const u32x4 kZeros = {0u, 0u, 0u, 0u};
+
+template <int PH_> struct Wide {
+    static constexpr int PH = PH_, kCols = 128 * PH, kRows = 256, kThreads = 512, FP = 4 * PH, FQ = 4;
+    static constexpr int kHalf = 128 * 128, kOperand = PH * kHalf, kStage = kOperand + 2 * kHalf, kLds = 2 * kStage;
+    // waves 0-3 and 4-7 have 64 columns of each half of P, a wave 32 rows of each half of Q
+    static __device__ __forceinline__ int p_piece(int wave, int i) { return (i >> 2) * 8 + (wave >> 2) * 4 + (i & 3); }
+    static __device__ __forceinline__ int q_piece(int wave, int j) { return (j >> 1) * 8 + (wave & 3) * 2 + (j & 1); }
+};
+
+__device__ __forceinline__ void to_lds(const void* g, char* l) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)g, (__attribute__((address_space(3))) uint32_t*)l, 16, 0, 0);
+}
+template <int N> __device__ __forceinline__ void wait_loads() {
+    static_assert(N == 0 || N == 4 || N == 6 || N == 10, "");
+    if constexpr (N == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if constexpr (N == 4) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+    if constexpr (N == 6) asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
+    if constexpr (N == 10) asm volatile("s_waitcnt vmcnt(10)" ::: "memory");
+}
+
+// Where the lanes of a wave read one operand's pieces, two pieces of 1 KB for each half: an address for the wave and 32 bits for the lane (a tile
+// spans less than 2 GB: launch_wide's rule), which is half the registers of whole addresses
+template <typename T, bool KC, int HALVES> struct Feed {
+    const char* base[HALVES];      // of the step that the half is asked for next
+    int64_t k[HALVES];             // its first contraction index
+    int64_t step;                  // bytes from step to step
+    uint32_t off[2 * HALVES];
+    int lane_k[2];                 // the lane's contraction index in a step, by piece
+
+    // PAIR: 16 rows of the first matrix, 16 of the second (KC).  Rows and columns behind the last are read from the last.
+    template <bool PAIR> __device__ __forceinline__ void begin(const void* m0, const void* m1, int64_t ld, int64_t first, int64_t count, int64_t k0) {
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const T* m = reinterpret_cast<const T*>(PAIR && (wave & 2) ? m1 : m0);      // (pieces `wave` and `wave + 8`: 16 rows are two pieces)
+        const char* start = reinterpret_cast<const char*>(m + (KC ? first * ld + k0 : k0 * ld + first));
+        step = (KC ? Kind<T>::kStep : Kind<T>::kStep * ld) * (int64_t)sizeof(T);
+        const int last = (int)(count - first < 256 ? count - first : 256) - 1;
+#pragma unroll
+        for (int i = 0; i < 2 * HALVES; ++i) {
+            const int half = i >> 1, piece = wave + 8 * (i & 1);
+            if constexpr (KC) {
+                const int r = half * 128 + piece * 8 + (lane >> 3), c = ((lane & 7) ^ (r & 7)) * Kind<T>::kPiece;
+                const int row = PAIR ? (r >> 5) * 16 + (r & 15) : r;
+                off[i] = ((uint32_t)(row < last ? row : last) * (uint32_t)ld + c) * (uint32_t)sizeof(T);
+                lane_k[i & 1] = c;
+            } else {
+                const int r = piece * 4 + (lane >> 4), slot = lane & 15, mask = (r & 3) | ((r >> 1) & 4);
+                const int col = half * 128 + ((((slot >> 1) ^ mask) << 1) | (slot & 1)) * 8;
+                off[i] = ((uint32_t)r * (uint32_t)ld + (col < last ? col : last - 7)) * (uint32_t)sizeof(T);
+                lane_k[i & 1] = r;
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) { base[h] = start; k[h] = k0; }
+    }
+    // asks for one half of its next step; the contraction ends at k1
+    __device__ __forceinline__ void ask(int half, char* lds, int64_t k1) {
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int left = k1 - k[half] < Kind<T>::kStep ? (int)(k1 - k[half]) : Kind<T>::kStep;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            char* to = lds + (wave + 8 * u) * 1024;
+            if (left == Kind<T>::kStep) to_lds(base[half] + off[half * 2 + u], to);
+            else to_lds(lane_k[u] < left ? base[half] + off[half * 2 + u] : reinterpret_cast<const char*>(&kZeros), to);
+        }
+        base[half] += step;
+        k[half] += Kind<T>::kStep;
+    }
+};
+
+template <typename T, int FORM, bool TWO, typename S> struct Stream {
+    static constexpr bool kPC = FORM == kForward, kQC = FORM != kWeightGrad;
+    using PT = Tile<T, kPC, 128, 512, true>;
+    using QT = Tile<T, kQC, 128, 512, true>;
+    Feed<T, kPC, S::PH> P;
+    Feed<T, kQC, 2> Q;
+    int64_t k1, K_first;
+    int64_t cross;      // kInputGrad with two weights: bytes from the end of the first to the start of the second
+
+    __device__ __forceinline__ void begin(const Args& a, int64_t p0, int64_t q0, int64_t k0, int64_t k_end) {
+        P.template begin<FORM == kForward && TWO>(a.P[0], a.P[1], a.p_ld, p0, a.p_count, k0);
+        Q.template begin<false>(a.Q, a.Q, a.q_ld, q0, a.q_count, k0);
+        k1 = k_end;
+        K_first = a.K_first;
+        if constexpr (FORM == kInputGrad && TWO)
+            cross = reinterpret_cast<const char*>(a.P[1]) - reinterpret_cast<const char*>(a.P[0]) - a.K_first * a.p_ld * (int64_t)sizeof(T);
+    }
+    __device__ __forceinline__ void ask_p(int half, char* stage) {
+        if constexpr (FORM == kInputGrad && TWO) {
+            if (P.k[half] == K_first) P.base[half] += cross;
+        }
+        P.ask(half, stage + half * S::kHalf, k1);
+    }
+    __device__ __forceinline__ void ask_q(int half, char* stage) { Q.ask(half, stage + S::kOperand + half * S::kHalf, k1); }
+    // what product() expects to have been asked for: the first step, and of the second all but what its first turn asks for
+    __device__ __forceinline__ void ask_first(char* lds, int64_t steps) {
+        ask_p(0, lds);
+        ask_q(0, lds);
+        ask_q(1, lds);
+        if constexpr (S::PH == 2) ask_p(1, lds);
+        if (steps > 1) {
+            ask_p(0, lds + S::kStage);
+            ask_q(0, lds + S::kStage);
+            if constexpr (S::PH == 2) ask_q(1, lds + S::kStage);
+        }
+    }
+
+    __device__ __forceinline__ void product(int64_t steps, char* lds, f32x4 (&acc)[S::FP][S::FQ]) {
+        constexpr int kBits = sizeof(T) == 1 ? 1 : 2;      // matrix instructions along a step
+        constexpr int kFlying = S::PH == 2 ? 10 : 6;
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wp = wave >> 2, wq = wave & 3;
+#pragma unroll
+        for (int i = 0; i < S::FP; ++i)
+#pragma unroll
+            for (int j = 0; j < S::FQ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        struct Operand { bf16x8 v[2]; };
+        if (wp == 1) __builtin_amdgcn_s_barrier();      // (from here on the two halves are a barrier apart)
+        char *cur = lds, *other = lds + S::kStage;
+        for (int64_t t = 0; t < steps; ++t) {
+            const bool more1 = t + 1 < steps, more2 = t + 2 < steps;
+            Operand x[4], y[2][2];
+            auto read_p = [&](int h) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (sizeof(T) == 1) x[i] = __builtin_bit_cast(Operand, PT::operand8(cur + h * S::kHalf, wp * 4 + i));
+                    else {
+#pragma unroll
+                        for (int s = 0; s < 2; ++s) x[i].v[s] = PT::operand(cur + h * S::kHalf, 0, wp * 4 + i, s);
+                    }
+                }
+            };
+            auto read_q = [&](int g) {
+                const char* at = cur + S::kOperand + g * S::kHalf;
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    if constexpr (sizeof(T) == 1) y[g][j] = __builtin_bit_cast(Operand, QT::operand8(at, wq * 2 + j));
+                    else {
+#pragma unroll
+                        for (int s = 0; s < 2; ++s) y[g][j].v[s] = QT::operand(at, 0, wq * 2 + j, s);
+                    }
+                }
+            };
+            auto wait = [&] {
+                if (more2) wait_loads<kFlying>();
+                else wait_loads<0>();
+            };
+            // The operands are in registers before the first barrier: behind it their place in LDS may be asked for again
+            auto multiply = [&](int h, int g) {
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                __builtin_amdgcn_sched_barrier(0);
+                __builtin_amdgcn_s_barrier();
+                __builtin_amdgcn_sched_barrier(0);
+                __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+                for (int s = 0; s < kBits; ++s)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            f32x4& c = acc[4 * h + i][2 * g + j];
+                            if constexpr (sizeof(T) == 1)
+                                c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_bit_cast(i32x8, x[i]), __builtin_bit_cast(i32x8, y[g][j]), c, 0, 0, 0, 0,
+                                                                                     0, 0);
+                            else
+                                c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[i].v[s], y[g][j].v[s], c, 0, 0, 0);
+                        }
+                __builtin_amdgcn_s_setprio(0);
+                __builtin_amdgcn_sched_barrier(0);
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            if constexpr (S::PH == 2) {
+                read_q(0);
+                read_p(0);
+                if (more1) ask_p(1, other);
+                wait();      // for this step's second half of Q
+                multiply(0, 0);
+                read_q(1);
+                if (more2) ask_p(0, cur);
+                wait();      // for its second half of P
+                multiply(0, 1);
+                read_p(1);
+                if (more2) ask_q(0, cur);
+                multiply(1, 0);
+                if (more2) ask_q(1, cur);
+                wait();      // for the first halves of the next step
+                multiply(1, 1);
+            } else {
+                read_q(0);
+                read_p(0);
+                if (more1) ask_q(1, other);
+                wait();
+                multiply(0, 0);
+                read_q(1);
+                if (more2) { ask_p(0, cur); ask_q(0, cur); }
+                wait();
+                multiply(0, 1);
+            }
+            char* c = cur;
+            cur = other;
+            other = c;
+        }
+        if (wp == 0) __builtin_amdgcn_s_barrier();
+    }
+};
 
 }  // namespace gemm
 }  // namespace tgt

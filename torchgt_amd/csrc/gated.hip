@@ -65,24 +65,17 @@ template <typename O> __device__ __forceinline__ void store4(O* p, int n, bool v
 }
 template <typename O> __device__ __forceinline__ bool fours(const void* p, int64_t ld) { return ((uintptr_t)p & (4 * sizeof(O) - 1)) == 0 && (ld & 3) == 0; }
 
-template <typename T, typename O, int FORM, bool TWO, bool GRAD, bool ALIGNED, typename S, int STAGES>
-__global__ __launch_bounds__(S::kThreads) void k_product(const Args a) {
-    extern __shared__ __attribute__((aligned(16))) char lds[];
+// What becomes of a tile's sums
+template <typename T, typename O, int FORM, bool TWO, bool GRAD, typename S>
+__device__ __forceinline__ void epilogue(const Args& a, int64_t p0, int64_t q0, unsigned split, const f32x4 (&acc)[S::FP][S::FQ]) {
     constexpr bool kPair = FORM == kForward && TWO;
-    unsigned tp, tq;
-    if (!tile_of(a, blockIdx.x, tp, tq)) return;
-    const int64_t p0 = (int64_t)tp * (kPair ? S::kCols / 2 : S::kCols), q0 = (int64_t)tq * S::kRows;
-    const int64_t k0 = (int64_t)blockIdx.y * a.K_each, k1 = k0 + a.K_each < a.K ? k0 + a.K_each : a.K;
-    f32x4 acc[S::FP][S::FQ];
-    product<T, FORM, TWO, ALIGNED, S, STAGES>(a, p0, q0, k0, k1, lds, acc);
-
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wp = wave % S::WP, wq = wave / S::WP;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     constexpr int kBy = kPair ? 2 : 1;      // pieces that one output piece takes
     constexpr bool EXACT = sizeof(O) == 4;
     const bool vec_out = fours<O>(a.out[0], a.out_ld) && (!a.out[1] || fours<O>(a.out[1], a.out_ld));
 #pragma unroll
     for (int i = 0; i < S::FP; i += kBy) {
-        const int64_t p = p0 + (wp * S::FP + i) / kBy * 16 + (lane >> 4) * 4;
+        const int64_t p = p0 + S::p_piece(wave, i) / kBy * 16 + (lane >> 4) * 4;
         if (p >= a.p_count) continue;
         const int n = a.p_count - p < 4 ? (int)(a.p_count - p) : 4;
         float bias[kBy][4], scale[kBy][4];
@@ -97,7 +90,7 @@ __global__ __launch_bounds__(S::kThreads) void k_product(const Args a) {
         }
 #pragma unroll
         for (int j = 0; j < S::FQ; ++j) {
-            const int64_t q = q0 + (wq * S::FQ + j) * 16 + (lane & 15);
+            const int64_t q = q0 + S::q_piece(wave, j) * 16 + (lane & 15);
             if (q >= a.q_count) continue;
             if constexpr (FORM == kForward) {
                 float v[kBy][4];
@@ -141,7 +134,7 @@ __global__ __launch_bounds__(S::kThreads) void k_product(const Args a) {
             } else {
                 const float o[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
                 if (FORM == kWeightGrad && a.partial) {
-                    float* to = a.partial + ((int64_t)blockIdx.y * a.q_count + q) * a.p_count + p;
+                    float* to = a.partial + ((int64_t)split * a.q_count + q) * a.p_count + p;
                     store4(to, n, fours<float>(a.partial, a.p_count), o);
                 } else if (FORM == kWeightGrad && q >= a.q_first) {
                     store4(reinterpret_cast<O*>(a.out[1]) + (q - a.q_first) * a.out_ld + p, n, vec_out, o);
@@ -150,6 +143,58 @@ __global__ __launch_bounds__(S::kThreads) void k_product(const Args a) {
                 }
             }
         }
+    }
+}
+
+
+template <typename T, typename O, int FORM, bool TWO, bool GRAD, bool ALIGNED, typename S, int STAGES>
+__global__ __launch_bounds__(S::kThreads) void k_product(const Args a) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    unsigned tp, tq;
+    if (!tile_of(a, blockIdx.x, tp, tq)) return;
+    const int64_t p0 = (int64_t)tp * (FORM == kForward && TWO ? S::kCols / 2 : S::kCols), q0 = (int64_t)tq * S::kRows;
+    const int64_t k0 = (int64_t)blockIdx.y * a.K_each, k1 = k0 + a.K_each < a.K ? k0 + a.K_each : a.K;
+    f32x4 acc[S::FP][S::FQ];
+    product<T, FORM, TWO, ALIGNED, S, STAGES>(a, p0, q0, k0, k1, lds, acc);
+    epilogue<T, O, FORM, TWO, GRAD, S>(a, p0, q0, blockIdx.y, acc);
+}
+
+// Large products: workgroup b takes the places b, b + gridDim.x, ... of the order of tiles (and splits); gridDim.x is a multiple of eight, so its
+// tiles stay on its XCD.  The next tile's first operands are asked for before this one's results are written.
+template <typename T, typename O, int FORM, bool TWO, bool GRAD, typename S>
+__global__ __launch_bounds__(S::kThreads, 2) void k_wide(const Args a, const unsigned places, const unsigned splits) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    struct Place { int64_t p0, q0, steps; unsigned split; };
+    Stream<T, FORM, TWO, S> stream;
+    Place now, next;
+    unsigned b = blockIdx.x;
+    auto find = [&](Place& at) {      // the next place that has a tile, its operands' addresses
+        for (; b < places * splits; b += gridDim.x) {
+            unsigned tp, tq;
+            at.split = b / places;
+            if (!tile_of(a, b % places, tp, tq)) continue;
+            at.p0 = (int64_t)tp * (FORM == kForward && TWO ? S::kCols / 2 : S::kCols);
+            at.q0 = (int64_t)tq * S::kRows;
+            const int64_t k0 = (int64_t)at.split * a.K_each, k1 = k0 + a.K_each < a.K ? k0 + a.K_each : a.K;
+            at.steps = (k1 - k0 + Kind<T>::kStep - 1) / Kind<T>::kStep;
+            stream.begin(a, at.p0, at.q0, k0, k1);
+            b += gridDim.x;
+            return true;
+        }
+        return false;
+    };
+    if (!find(next)) return;
+    stream.ask_first(lds, next.steps);
+    for (bool more = true; more;) {
+        now = next;
+        wait_loads<0>();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        f32x4 acc[S::FP][S::FQ];
+        stream.product(now.steps, lds, acc);
+        more = find(next);
+        if (more) stream.ask_first(lds, next.steps);
+        epilogue<T, O, FORM, TWO, GRAD, S>(a, now.p0, now.q0, now.split, acc);
     }
 }
 
@@ -206,6 +251,29 @@ int launch(Args a, int splits, hipStream_t st) {
     return TGT_OK;
 }
 
+template <typename T, typename O, int FORM, bool TWO, bool GRAD, typename S>
+int launch_wide(Args a, int splits, hipStream_t st) {
+    constexpr int kCols = FORM == kForward && TWO ? S::kCols / 2 : S::kCols;
+    a.p_tiles = (unsigned)((a.p_count + kCols - 1) / kCols);
+    a.q_tiles = (unsigned)((a.q_count + S::kRows - 1) / S::kRows);
+    const int64_t places = ((int64_t)a.p_tiles * a.q_tiles + 7) / 8 * 8;
+    if (places * splits > (1ll << 30)) { set_error("torchgt: a product of more than 2^30 tiles"); return TGT_ERR_UNSUPPORTED; }
+    auto* kernel = k_wide<T, O, FORM, TWO, GRAD, S>;
+    static std::atomic<uint64_t> done{0};
+    const int rc = allow_lds((const void*)kernel, S::kLds, done);
+    if (rc != TGT_OK) return rc;
+    const unsigned grid = (unsigned)std::min<int64_t>(places * splits, num_cus() / 8 * 8);
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(S::kThreads), S::kLds, st, a, (unsigned)places, (unsigned)splits);
+    TGT_HIP_CHECK(hipGetLastError());
+    return TGT_OK;
+}
+
+// Tiles of `cols` x 256 that keep the CUs busy
+bool wide_enough(const Args& a, int cols, int splits) {
+    const int64_t tiles = (a.p_count + cols - 1) / cols * ((a.q_count + 255) / 256) * splits;
+    return tiles >= 200 && a.K >= 256 && a.p_ld < (1 << 21) && a.q_ld < (1 << 21);
+}
+
 bool aligned16(const void* p, int64_t ld, int size) { return ((uintptr_t)p & 15) == 0 && ld * size % 16 == 0; }
 
 }  // namespace
@@ -220,6 +288,14 @@ template <typename T, typename O> int product_forward(const Args& a, bool grad, 
     constexpr int kStages = sizeof(T) == 4 ? 1 : 2;
     const bool two = a.P[1] != nullptr;
     const bool al = aligned16(a.Q, a.q_ld, sizeof(T)) && aligned16(a.P[0], a.p_ld, sizeof(T)) && (!two || aligned16(a.P[1], a.p_ld, sizeof(T)));
+    if constexpr (sizeof(T) < 4) {
+        if (al && wide_enough(a, two ? 128 : 256, 1)) {
+#define X(TWO, GRAD) if (two == TWO && grad == GRAD) return launch_wide<T, O, kForward, TWO, GRAD, Wide<2>>(a, 1, st)
+            X(false, false); X(true, false);
+            if constexpr (sizeof(T) > 1) { X(false, true); X(true, true); }
+#undef X
+        }
+    }
 #define X(TWO, GRAD, AL) if (two == TWO && grad == GRAD && al == AL) return launch<T, O, kForward, TWO, GRAD, AL, Square, kStages>(a, 1, st)
     X(false, false, true); X(true, false, true); X(false, false, false); X(true, false, false);
     if constexpr (sizeof(T) > 1) { X(false, true, true); X(true, true, true); X(false, true, false); X(true, true, false); }
@@ -232,6 +308,12 @@ template <typename T> int product_input_grad(const Args& a, hipStream_t st) {
     constexpr int kStages = sizeof(T) == 4 ? 1 : 2;
     const bool two = a.P[1] != nullptr;
     const bool al = aligned16(a.Q, a.q_ld, sizeof(T)) && aligned16(a.P[0], a.p_ld, sizeof(T)) && (!two || aligned16(a.P[1], a.p_ld, sizeof(T)));
+    if constexpr (sizeof(T) < 4) {
+        if (al && a.p_count % 8 == 0 && (!two || a.K_first % Kind<T>::kStep == 0) && wide_enough(a, 256, 1)) {
+            if (two) return launch_wide<T, T, kInputGrad, true, false, Wide<2>>(a, 1, st);
+            return launch_wide<T, T, kInputGrad, false, false, Wide<2>>(a, 1, st);
+        }
+    }
 #define X(TWO, AL) if (two == TWO && al == AL) return launch<T, T, kInputGrad, TWO, false, AL, Square, kStages>(a, 1, st)
     X(false, true); X(true, true); X(false, false); X(true, false);
 #undef X
@@ -239,7 +321,14 @@ template <typename T> int product_input_grad(const Args& a, hipStream_t st) {
 }
 template <typename T> int product_weight_grad(const Args& a, int splits, hipStream_t st) {
     constexpr int kStages = sizeof(T) == 4 ? 1 : 2;
-    if (aligned16(a.Q, a.q_ld, sizeof(T)) && aligned16(a.P[0], a.p_ld, sizeof(T))) return launch<T, T, kWeightGrad, false, false, true, Square, kStages>(a, splits, st);
+    const bool al = aligned16(a.Q, a.q_ld, sizeof(T)) && aligned16(a.P[0], a.p_ld, sizeof(T));
+    if constexpr (sizeof(T) < 4) {
+        if (al && a.p_count % 8 == 0 && a.q_count % 8 == 0) {
+            if (wide_enough(a, 256, splits)) return launch_wide<T, T, kWeightGrad, false, false, Wide<2>>(a, splits, st);
+            if (wide_enough(a, 128, splits)) return launch_wide<T, T, kWeightGrad, false, false, Wide<1>>(a, splits, st);
+        }
+    }
+    if (al) return launch<T, T, kWeightGrad, false, false, true, Square, kStages>(a, splits, st);
     return launch<T, T, kWeightGrad, false, false, false, Square, kStages>(a, splits, st);
 }
 #endif
