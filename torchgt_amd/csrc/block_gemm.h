@@ -17,6 +17,7 @@
 // plain multiply-adds.
 #pragma once
 #include "common.h"
+#include <type_traits>
 
 namespace tgt {
 namespace gemm {
@@ -391,43 +392,49 @@ __device__ __forceinline__ bool tile_of(const Args& a, unsigned b, unsigned& tp,
 
 // ---- large products of 16- and 8-bit operands ----------------------------------------------------------------------------------------
 //
-// Eight waves, 128 PH x 256 of the result, one workgroup to a CU that goes from tile to tile.  Operands go from memory straight to LDS
-// (global_load_lds, 16 bytes a lane), two steps deep; each half of an operand's tile (16 KB) is asked for again as soon as the
-// whole workgroup has read it, nearly two steps ahead.  Waves 0-3 and 4-7 - on each SIMD one of either - run one barrier apart: while one half of
-// them multiplies, the other reads its next operands from LDS.  A step has PH x 2 turns of 16 matrix instructions; a wave's counter of
-// outstanding loads is waited down to what was asked for after the halves that the next turn reads, so loads stay in flight over every barrier.
+// Eight waves, 128 PH x 256 of the result, one workgroup to a CU that goes from tile to tile.  Operands go from memory straight to LDS, 16 KB (one half of an
+// operand's tile) at a time, and each place is asked for again as soon as all waves have read it: about one and a half steps ahead.  A step
+// is cut into turns of 16 matrix instructions that need only what is in registers; a turn's operands are read from LDS during the turn before.
+// Two barriers a step; a wave's counter of outstanding loads is waited down to the newest requests only, so loads stay in flight over every barrier.
 //
-// A contraction that ends inside a step reads zeros for the rest: lanes past its end are pointed at 16 bytes of them.
-
-static __device__ const u32x4 kZeros = {0u, 0u, 0u, 0u};
+// Measured, 8192 x 8192 x 8192 bf16 (torch.mm 1422 TFLOP/s): 778 us, 1414 TFLOP/s.  A wave that works on 128 x 64 reads 24 KB from LDS for 64 matrix
+// instructions; with neither requests nor reads of LDS the same loop takes 629 us, with reads only 755.  Before: operands through registers, one step ahead 1324 us;
+// straight to LDS with the operands of each turn read in front of it, the two halves of the workgroup a barrier apart 937.
+//
+// A contraction that ends inside a step: what is left of it goes through registers, zeros behind its end.
 
 template <int PH_> struct Wide {
     static constexpr int PH = PH_, kCols = 128 * PH, kRows = 256, kThreads = 512, FP = 4 * PH, FQ = 4;
-    static constexpr int kHalf = 128 * 128, kOperand = PH * kHalf, kStage = kOperand + 2 * kHalf, kLds = 2 * kStage;
+    static constexpr int kHalf = 128 * 128, kOperand = PH * kHalf, kStage = kOperand + 2 * kHalf, kStages = PH == 2 ? 2 : 3, kLds = kStages * kStage;
     // waves 0-3 and 4-7 have 64 columns of each half of P, a wave 32 rows of each half of Q
     static __device__ __forceinline__ int p_piece(int wave, int i) { return (i >> 2) * 8 + (wave >> 2) * 4 + (i & 3); }
     static __device__ __forceinline__ int q_piece(int wave, int j) { return (j >> 1) * 8 + (wave & 3) * 2 + (j & 1); }
 };
 
-__device__ __forceinline__ void to_lds(const void* g, char* l) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)g, (__attribute__((address_space(3))) uint32_t*)l, 16, 0, 0);
+// 16 bytes for each lane, from an address of the wave and 32 bits of the lane's, to 1 KB of LDS at byte `at`.  A buffer instruction: with a global one the
+// compiler keeps a whole address per lane and request and adds the step to each.  Written out: behind the builtin the compiler waits for
+// every such load before the next transposed read, whatever it reads (ds_read_b64_tr_b16; input gradient of 16384 x 8192 x 1024: 318 us).  The
+// instruction has no result registers; whoever reads what it brings waits with wait_loads().  m0 has no other use in these kernels.
+__device__ __forceinline__ void to_lds(const char* base, uint32_t off, uint32_t at) {
+    typedef uint32_t u32x4s __attribute__((ext_vector_type(4)));
+    const uint64_t b = (uint64_t)(uintptr_t)base;
+    const u32x4s r = {(uint32_t)b, (uint32_t)(b >> 32), 0xffffffffu, 0x00020000u};      // (a plain buffer of bytes)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(off), "s"(r) : "memory");
 }
+__device__ __forceinline__ uint32_t lds_byte(const char* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p; }
 template <int N> __device__ __forceinline__ void wait_loads() {
-    static_assert(N == 0 || N == 4 || N == 6 || N == 10, "");
+    static_assert(N == 0 || N == 6 || N == 8, "");
     if constexpr (N == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if constexpr (N == 4) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
     if constexpr (N == 6) asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
-    if constexpr (N == 10) asm volatile("s_waitcnt vmcnt(10)" ::: "memory");
+    if constexpr (N == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
 }
 
 // Where the lanes of a wave read one operand's pieces, two pieces of 1 KB for each half: an address for the wave and 32 bits for the lane (a tile
-// spans less than 2 GB: launch_wide's rule), which is half the registers of whole addresses
+// spans less than 2 GB: the rule for these kernels), which is half the registers of whole addresses
 template <typename T, bool KC, int HALVES> struct Feed {
     const char* base[HALVES];      // of the step that the half is asked for next
-    int64_t k[HALVES];             // its first contraction index
     int64_t step;                  // bytes from step to step
     uint32_t off[2 * HALVES];
-    int lane_k[2];                 // the lane's contraction index in a step, by piece
 
     // PAIR: 16 rows of the first matrix, 16 of the second (KC).  Rows and columns behind the last are read from the last.
     template <bool PAIR> __device__ __forceinline__ void begin(const void* m0, const void* m1, int64_t ld, int64_t first, int64_t count, int64_t k0) {
@@ -443,29 +450,21 @@ template <typename T, bool KC, int HALVES> struct Feed {
                 const int r = half * 128 + piece * 8 + (lane >> 3), c = ((lane & 7) ^ (r & 7)) * Kind<T>::kPiece;
                 const int row = PAIR ? (r >> 5) * 16 + (r & 15) : r;
                 off[i] = ((uint32_t)(row < last ? row : last) * (uint32_t)ld + c) * (uint32_t)sizeof(T);
-                lane_k[i & 1] = c;
             } else {
                 const int r = piece * 4 + (lane >> 4), slot = lane & 15, mask = (r & 3) | ((r >> 1) & 4);
                 const int col = half * 128 + ((((slot >> 1) ^ mask) << 1) | (slot & 1)) * 8;
                 off[i] = ((uint32_t)r * (uint32_t)ld + (col < last ? col : last - 7)) * (uint32_t)sizeof(T);
-                lane_k[i & 1] = r;
             }
         }
 #pragma unroll
-        for (int h = 0; h < HALVES; ++h) { base[h] = start; k[h] = k0; }
+        for (int h = 0; h < HALVES; ++h) base[h] = start;
     }
-    // asks for one half of its next step; the contraction ends at k1
-    __device__ __forceinline__ void ask(int half, char* lds, int64_t k1) {
+    // asks for one half of its next step
+    __device__ __forceinline__ void ask(int half, char* lds) {
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        const int left = k1 - k[half] < Kind<T>::kStep ? (int)(k1 - k[half]) : Kind<T>::kStep;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            char* to = lds + (wave + 8 * u) * 1024;
-            if (left == Kind<T>::kStep) to_lds(base[half] + off[half * 2 + u], to);
-            else to_lds(lane_k[u] < left ? base[half] + off[half * 2 + u] : reinterpret_cast<const char*>(&kZeros), to);
-        }
+        for (int u = 0; u < 2; ++u) to_lds(base[half], off[half * 2 + u], lds_byte(lds) + (wave + 8 * u) * 1024);
         base[half] += step;
-        k[half] += Kind<T>::kStep;
     }
 };
 
@@ -475,134 +474,186 @@ template <typename T, int FORM, bool TWO, typename S> struct Stream {
     using QT = Tile<T, kQC, 128, 512, true>;
     Feed<T, kPC, S::PH> P;
     Feed<T, kQC, 2> Q;
-    int64_t k1, K_first;
-    int64_t cross;      // kInputGrad with two weights: bytes from the end of the first to the start of the second
+    int64_t cross;               // kInputGrad with two weights: bytes from the end of the first to the start of the second,
+    int64_t until[S::PH];        // and steps until a half of P gets there
 
-    __device__ __forceinline__ void begin(const Args& a, int64_t p0, int64_t q0, int64_t k0, int64_t k_end) {
+    __device__ __forceinline__ void begin(const Args& a, int64_t p0, int64_t q0, int64_t k0) {
         P.template begin<FORM == kForward && TWO>(a.P[0], a.P[1], a.p_ld, p0, a.p_count, k0);
         Q.template begin<false>(a.Q, a.Q, a.q_ld, q0, a.q_count, k0);
-        k1 = k_end;
-        K_first = a.K_first;
-        if constexpr (FORM == kInputGrad && TWO)
+        if constexpr (FORM == kInputGrad && TWO) {
             cross = reinterpret_cast<const char*>(a.P[1]) - reinterpret_cast<const char*>(a.P[0]) - a.K_first * a.p_ld * (int64_t)sizeof(T);
+#pragma unroll
+            for (int h = 0; h < S::PH; ++h) until[h] = a.K_first / Kind<T>::kStep;
+        }
     }
     __device__ __forceinline__ void ask_p(int half, char* stage) {
         if constexpr (FORM == kInputGrad && TWO) {
-            if (P.k[half] == K_first) P.base[half] += cross;
+            if (until[half]-- == 0) P.base[half] += cross;
         }
-        P.ask(half, stage + half * S::kHalf, k1);
+        P.ask(half, stage + half * S::kHalf);
     }
-    __device__ __forceinline__ void ask_q(int half, char* stage) { Q.ask(half, stage + S::kOperand + half * S::kHalf, k1); }
-    // what product() expects to have been asked for: the first step, and of the second all but what its first turn asks for
+    __device__ __forceinline__ void ask_q(int half, char* stage) { Q.ask(half, stage + S::kOperand + half * S::kHalf); }
+    // One step of the second half of P is asked for apart from the rest, when the waves have read the one before
+    __device__ __forceinline__ void ask_early(int part, char* stage) {      // part 0: two halves, part 1: the last
+        if (part == 0) { ask_p(0, stage); ask_q(0, stage); }
+        else ask_q(1, stage);
+    }
+    // what product() expects to have been asked for: as many steps as there are places
     __device__ __forceinline__ void ask_first(char* lds, int64_t steps) {
-        ask_p(0, lds);
-        ask_q(0, lds);
-        ask_q(1, lds);
-        if constexpr (S::PH == 2) ask_p(1, lds);
-        if (steps > 1) {
-            ask_p(0, lds + S::kStage);
-            ask_q(0, lds + S::kStage);
-            if constexpr (S::PH == 2) ask_q(1, lds + S::kStage);
+        for (int i = 0; i < S::kStages && i < steps; ++i) {
+            ask_early(0, lds + i * S::kStage);
+            ask_early(1, lds + i * S::kStage);
+            if constexpr (S::PH == 2) ask_p(1, lds + i * S::kStage);
         }
     }
 
+    struct Operand { bf16x8 v[2]; };
+    __device__ __forceinline__ void read_p(Operand& x, const char* stage, int h, int i, int wp) const {
+        if constexpr (sizeof(T) == 1) x = __builtin_bit_cast(Operand, PT::operand8(stage + h * S::kHalf, wp * 4 + i));
+        else {
+#pragma unroll
+            for (int s = 0; s < 2; ++s) x.v[s] = PT::operand(stage + h * S::kHalf, 0, wp * 4 + i, s);
+        }
+    }
+    __device__ __forceinline__ void read_q(Operand (&y)[2], const char* stage, int g, int wq) const {
+        const char* at = stage + S::kOperand + g * S::kHalf;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            if constexpr (sizeof(T) == 1) y[j] = __builtin_bit_cast(Operand, QT::operand8(at, wq * 2 + j));
+            else {
+#pragma unroll
+                for (int s = 0; s < 2; ++s) y[j].v[s] = QT::operand(at, 0, wq * 2 + j, s);
+            }
+        }
+    }
+    // One turn.  `after(i)` is called when x[i] has been used for the last time: its registers may take the next operand.  (Two rows of pieces side by side: four
+    // products lie between two that add to the same sum.)
+    template <int H, int G, typename A> __device__ __forceinline__ void multiply(const Operand (&x)[4], const Operand (&y)[2], f32x4 (&acc)[S::FP][S::FQ], A after) const {
+#pragma unroll
+        for (int i0 = 0; i0 < 4; i0 += 2) {
+#pragma unroll
+            for (int s = 0; s < (sizeof(T) == 1 ? 1 : 2); ++s)
+#pragma unroll
+                for (int i = i0; i < i0 + 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        f32x4& c = acc[4 * H + i][2 * G + j];
+                        if constexpr (sizeof(T) == 1)
+                            c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_bit_cast(i32x8, x[i]), __builtin_bit_cast(i32x8, y[j]), c, 0, 0, 0, 0, 0, 0);
+                        else
+                            c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[i].v[s], y[j].v[s], c, 0, 0, 0);
+                    }
+            __builtin_amdgcn_sched_barrier(0);
+            after(i0);
+            after(i0 + 1);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    // Every wave's operands read so far are in registers, and what was asked for before the newest `flying` requests has come, for all waves
+    __device__ __forceinline__ void meet(bool flying) const {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (flying) wait_loads<S::PH == 2 ? 8 : 6>();
+        else wait_loads<0>();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    // Step t: x holds the first half of P, y0 that of Q; in the end x and y1 (one half of P: x and y0) hold the next step's (of the last step: nothing of
+    // use).  A turn needs only what is in registers, and each operand is read as soon as the registers that it goes to have been used for
+    // the last time.  INNER: there are kStages steps more.
+    template <bool INNER>
+    __device__ __forceinline__ void step(int64_t t, int64_t steps, char* cur, char* next, Operand (&x)[4], Operand (&y0)[2], Operand (&y1)[2], int wp, int wq,
+                                         f32x4 (&acc)[S::FP][S::FQ]) {
+        const bool ask = INNER || t + S::kStages < steps, flying = INNER || t + 2 < steps;
+        auto nothing = [](int) {};
+        auto next_p = [&](int i) { read_p(x[i], next, 0, i, wp); };
+        read_q(y1, cur, 1, wq);
+        multiply<0, 0>(x, y0, acc, nothing);
+        meet(flying);
+        if constexpr (S::PH == 2) {
+            if (ask) ask_early(0, cur);
+            multiply<0, 1>(x, y1, acc, [&](int i) { read_p(x[i], cur, 1, i, wp); });
+            if (ask) ask_early(1, cur);
+            multiply<1, 1>(x, y1, acc, nothing);
+            meet(flying);
+            read_q(y1, next, 0, wq);
+            if (ask) ask_p(1, cur);
+            multiply<1, 0>(x, y0, acc, next_p);
+        } else {
+            read_q(y0, next, 0, wq);
+            if (ask) { ask_early(0, cur); ask_early(1, cur); }
+            multiply<0, 1>(x, y1, acc, next_p);
+        }
+    }
     __device__ __forceinline__ void product(int64_t steps, char* lds, f32x4 (&acc)[S::FP][S::FQ]) {
-        constexpr int kBits = sizeof(T) == 1 ? 1 : 2;      // matrix instructions along a step
-        constexpr int kFlying = S::PH == 2 ? 10 : 6;
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wp = wave >> 2, wq = wave & 3;
 #pragma unroll
         for (int i = 0; i < S::FP; ++i)
 #pragma unroll
             for (int j = 0; j < S::FQ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-        struct Operand { bf16x8 v[2]; };
-        if (wp == 1) __builtin_amdgcn_s_barrier();      // (from here on the two halves are a barrier apart)
-        char *cur = lds, *other = lds + S::kStage;
-        for (int64_t t = 0; t < steps; ++t) {
-            const bool more1 = t + 1 < steps, more2 = t + 2 < steps;
-            Operand x[4], y[2][2];
-            auto read_p = [&](int h) {
+        if (steps == 0) return;
+        Operand x[4], y0[2], y1[2];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if constexpr (sizeof(T) == 1) x[i] = __builtin_bit_cast(Operand, PT::operand8(cur + h * S::kHalf, wp * 4 + i));
-                    else {
-#pragma unroll
-                        for (int s = 0; s < 2; ++s) x[i].v[s] = PT::operand(cur + h * S::kHalf, 0, wp * 4 + i, s);
-                    }
-                }
-            };
-            auto read_q = [&](int g) {
-                const char* at = cur + S::kOperand + g * S::kHalf;
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    if constexpr (sizeof(T) == 1) y[g][j] = __builtin_bit_cast(Operand, QT::operand8(at, wq * 2 + j));
-                    else {
-#pragma unroll
-                        for (int s = 0; s < 2; ++s) y[g][j].v[s] = QT::operand(at, 0, wq * 2 + j, s);
-                    }
-                }
-            };
-            auto wait = [&] {
-                if (more2) wait_loads<kFlying>();
-                else wait_loads<0>();
-            };
-            // The operands are in registers before the first barrier: behind it their place in LDS may be asked for again
-            auto multiply = [&](int h, int g) {
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                __builtin_amdgcn_sched_barrier(0);
-                __builtin_amdgcn_s_barrier();
-                __builtin_amdgcn_sched_barrier(0);
-                __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-                for (int s = 0; s < kBits; ++s)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            f32x4& c = acc[4 * h + i][2 * g + j];
-                            if constexpr (sizeof(T) == 1)
-                                c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_bit_cast(i32x8, x[i]), __builtin_bit_cast(i32x8, y[g][j]), c, 0, 0, 0, 0,
-                                                                                     0, 0);
-                            else
-                                c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[i].v[s], y[g][j].v[s], c, 0, 0, 0);
-                        }
-                __builtin_amdgcn_s_setprio(0);
-                __builtin_amdgcn_sched_barrier(0);
-                __builtin_amdgcn_s_barrier();
-                asm volatile("" ::: "memory");
-                __builtin_amdgcn_sched_barrier(0);
-            };
-            if constexpr (S::PH == 2) {
-                read_q(0);
-                read_p(0);
-                if (more1) ask_p(1, other);
-                wait();      // for this step's second half of Q
-                multiply(0, 0);
-                read_q(1);
-                if (more2) ask_p(0, cur);
-                wait();      // for its second half of P
-                multiply(0, 1);
-                read_p(1);
-                if (more2) ask_q(0, cur);
-                multiply(1, 0);
-                if (more2) ask_q(1, cur);
-                wait();      // for the first halves of the next step
-                multiply(1, 1);
-            } else {
-                read_q(0);
-                read_p(0);
-                if (more1) ask_q(1, other);
-                wait();
-                multiply(0, 0);
-                read_q(1);
-                if (more2) { ask_p(0, cur); ask_q(0, cur); }
-                wait();
-                multiply(0, 1);
-            }
+        for (int i = 0; i < 4; ++i) read_p(x[i], lds, 0, i, wp);
+        read_q(y0, lds, 0, wq);
+        char *cur = lds, *next = lds + S::kStage, *then = lds + (S::kStages - 1) * S::kStage;
+        auto turn = [&] {
             char* c = cur;
-            cur = other;
-            other = c;
+            cur = next;
+            next = S::kStages == 2 ? c : then;
+            then = c;
+        };
+        int64_t t = 0;
+        auto two = [&](auto inner) {
+            constexpr bool INNER = decltype(inner)::value;
+            step<INNER>(t, steps, cur, next, x, y0, y1, wp, wq, acc);
+            turn();
+            if (INNER || t + 1 < steps) {
+                if constexpr (S::PH == 2) step<INNER>(t + 1, steps, cur, next, x, y1, y0, wp, wq, acc);
+                else step<INNER>(t + 1, steps, cur, next, x, y0, y1, wp, wq, acc);
+                turn();
+            }
+            t += 2;
+        };
+        while (t + 1 + S::kStages < steps) two(std::true_type{});
+        while (t < steps) two(std::false_type{});
+        __builtin_amdgcn_s_barrier();      // (the last operands have been read: the places may be asked for again)
+        asm volatile("" ::: "memory");
+    }
+    // What is left behind the last whole step: contraction indices k .. k1 - 1
+    __device__ __forceinline__ void rest(const Args& a, int64_t p0, int64_t q0, int64_t k, int64_t k1, char* lds, f32x4 (&acc)[S::FP][S::FQ]) {
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wp = wave >> 2, wq = wave & 3;
+        const void* qs[2] = {a.Q, a.Q};
+        constexpr bool kPair = FORM == kForward && TWO;
+#pragma unroll
+        for (int h = 0; h < S::PH; ++h) {
+            PT t;
+            t.template begin<kPair>(a.P, a.p_ld, p0 + h * (kPair ? 64 : 128), a.p_count);
+            if constexpr (kPC) t.fetch_contiguous(k, k1);
+            else t.template fetch_rows<FORM == kInputGrad && TWO>(a.P, a.p_ld, p0 + h * 128, a.p_count, k, k1, a.K_first);
+            t.store(lds + h * S::kHalf);
         }
-        if (wp == 0) __builtin_amdgcn_s_barrier();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            QT t;
+            t.template begin<false>(qs, a.q_ld, q0 + h * 128, a.q_count);
+            if constexpr (kQC) t.fetch_contiguous(k, k1);
+            else t.template fetch_rows<false>(qs, a.q_ld, q0 + h * 128, a.q_count, k, k1, k1);
+            t.store(lds + S::kOperand + h * S::kHalf);
+        }
+        __syncthreads();
+        Operand x[4], y[2][2];
+        auto nothing = [](int) {};
+        read_q(y[0], lds, 0, wq);
+        read_q(y[1], lds, 1, wq);
+#pragma unroll
+        for (int h = 0; h < S::PH; ++h) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) read_p(x[i], lds, h, i, wp);
+            if (h == 0) { multiply<0, 0>(x, y[0], acc, nothing); multiply<0, 1>(x, y[1], acc, nothing); }
+            else { multiply<S::PH - 1, 0>(x, y[0], acc, nothing); multiply<S::PH - 1, 1>(x, y[1], acc, nothing); }
+        }
+        __syncthreads();
     }
 };
 

@@ -18,80 +18,106 @@ namespace {
 
 using namespace gemm;
 
-// act(u), and dh * act'(u).  SILU: u / (1 + exp(-u))
-template <bool EXACT> __device__ __forceinline__ float exp_of(float v) { return EXACT ? expf(v) : __expf(v); }
-template <bool EXACT> __device__ __forceinline__ float act_of(int act, float u) {
-    if (act == TGT_ACT_SILU) return u / (1.f + exp_of<EXACT>(-u));
-    if (act == TGT_ACT_GELU) return act_value<false>(u);
-    if (act == TGT_ACT_RELU) return act_value<true>(u);
+// act(u), and dh * act'(u).  SILU: u / (1 + exp(-u)); EXACT (float32 results): with expf and a division, else with the hardware's exp2 and reciprocal, which are
+// good to 2^-22 and 2^-14 |u| of a result of 8 bits
+template <bool EXACT> __device__ __forceinline__ float sigmoid_of(float u) {
+    return EXACT ? 1.f / (1.f + expf(-u)) : __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(u * -1.4426950408889634f));
+}
+template <bool EXACT, int ACT> __device__ __forceinline__ float act_of(float u) {
+    if (ACT == TGT_ACT_SILU) return EXACT ? u / (1.f + expf(-u)) : u * sigmoid_of<false>(u);
+    if (ACT == TGT_ACT_GELU) return act_value<false>(u);
+    if (ACT == TGT_ACT_RELU) return act_value<true>(u);
     return u;
 }
-template <bool EXACT> __device__ __forceinline__ float slope_of(int act, float u, float dh) {
-    if (act == TGT_ACT_SILU) {
-        const float s = 1.f / (1.f + exp_of<EXACT>(-u));
+template <bool EXACT, int ACT> __device__ __forceinline__ float slope_of(float u, float dh) {
+    if (ACT == TGT_ACT_SILU) {
+        const float s = sigmoid_of<EXACT>(u);
         return dh * (s * (1.f + u * (1.f - s)));
     }
-    if (act == TGT_ACT_GELU) return act_grad<false>(u, dh);
-    if (act == TGT_ACT_RELU) return act_grad<true>(u, dh);
+    if (ACT == TGT_ACT_GELU) return act_grad<false>(u, dh);
+    if (ACT == TGT_ACT_RELU) return act_grad<true>(u, dh);
     return dh;
 }
 
-// Four neighbouring elements of a row, `n` of which exist; vec: the row is aligned for one access
-template <typename O> __device__ __forceinline__ void load4(const O* p, int n, bool vec, float (&f)[4]) {
-    O e[4] = {};
-    if (vec && n >= 4) {
-        if constexpr (sizeof(O) == 4) *reinterpret_cast<u32x4*>(e) = *reinterpret_cast<const u32x4*>(p);
-        else *reinterpret_cast<uint2*>(e) = *reinterpret_cast<const uint2*>(p);
-    } else {
+// Four neighbouring elements of a row in memory
+template <typename O> struct Four { O e[4]; };
+template <> struct Four<b16> { union { b16 e[4]; uint2 v; }; };
+template <> struct Four<float> { union { float e[4]; u32x4 v; }; };
+// WHOLE: all four exist and the address is aligned to them; else the first n do
+template <typename O, bool WHOLE> __device__ __forceinline__ Four<O> load4(const O* p, int n) {
+    Four<O> f;
+    if constexpr (WHOLE) f.v = *reinterpret_cast<const decltype(f.v)*>(p);
+    else {
+        f.v = decltype(f.v){};
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (i < n) e[i] = p[i];
+            if (i < n) f.e[i] = p[i];
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = to_float(e[i]);
+    return f;
 }
-template <typename O> __device__ __forceinline__ void store4(O* p, int n, bool vec, const float (&f)[4]) {
-    O e[4];
+template <typename O, bool WHOLE> __device__ __forceinline__ void store4(O* p, int n, const float (&v)[4]) {
+    Four<O> f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) from_float(e[i], f[i]);
-    if (vec && n >= 4) {
-        if constexpr (sizeof(O) == 4) *reinterpret_cast<u32x4*>(p) = *reinterpret_cast<const u32x4*>(e);
-        else *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(e);
-    } else {
+    for (int i = 0; i < 4; ++i) from_float(f.e[i], v[i]);
+    if constexpr (WHOLE) *reinterpret_cast<decltype(f.v)*>(p) = f.v;
+    else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (i < n) p[i] = e[i];
+            if (i < n) p[i] = f.e[i];
     }
 }
 template <typename O> __device__ __forceinline__ bool fours(const void* p, int64_t ld) { return ((uintptr_t)p & (4 * sizeof(O) - 1)) == 0 && (ld & 3) == 0; }
 
-// What becomes of a tile's sums
-template <typename T, typename O, int FORM, bool TWO, bool GRAD, typename S>
-__device__ __forceinline__ void epilogue(const Args& a, int64_t p0, int64_t q0, unsigned split, const f32x4 (&acc)[S::FP][S::FQ]) {
-    constexpr bool kPair = FORM == kForward && TWO;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    constexpr int kBy = kPair ? 2 : 1;      // pieces that one output piece takes
-    constexpr bool EXACT = sizeof(O) == 4;
-    const bool vec_out = fours<O>(a.out[0], a.out_ld) && (!a.out[1] || fours<O>(a.out[1], a.out_ld));
+// What becomes of a tile's sums.  WHOLE: the tile lies inside the result and all rows are aligned to four elements; what is read is then asked for
+// before the first value is formed.
+template <typename T, typename O, int FORM, bool TWO, bool GRAD, typename S, int ACT, bool WHOLE>
+__device__ __forceinline__ void finish(const Args& a, int64_t p0, int64_t q0, unsigned split, const f32x4 (&acc)[S::FP][S::FQ]) {
+    constexpr bool kPair = FORM == kForward && TWO, EXACT = sizeof(O) == 4, kReads = FORM == kForward && (GRAD || !TWO);
+    constexpr int kBy = kPair ? 2 : 1, kOut = S::FP / kBy;      // pieces that one output piece takes
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = (lane >> 4) * 4, row = lane & 15;
+    const O* more = reinterpret_cast<const O*>(GRAD ? a.dy : a.residual);
+    int left[kOut];
 #pragma unroll
-    for (int i = 0; i < S::FP; i += kBy) {
-        const int64_t p = p0 + S::p_piece(wave, i) / kBy * 16 + (lane >> 4) * 4;
-        if (p >= a.p_count) continue;
-        const int n = a.p_count - p < 4 ? (int)(a.p_count - p) : 4;
+    for (int i = 0; i < kOut; ++i) {
+        const int64_t n = a.p_count - (p0 + S::p_piece(wave, i * kBy) / kBy * 16 + col);
+        left[i] = n < 4 ? (int)n : 4;
+    }
+    Four<O> in[kReads ? kOut : 1][S::FQ];
+    if (kReads && more) {
+#pragma unroll
+        for (int j = 0; j < S::FQ; ++j) {
+            const int64_t q = q0 + S::q_piece(wave, j) * 16 + row;
+            const O* from = more + q * a.p_count + p0 + col;
+#pragma unroll
+            for (int i = 0; i < kOut; ++i) in[kReads ? i : 0][j] = load4<O, WHOLE>(from + S::p_piece(wave, i * kBy) / kBy * 16, q < a.q_count ? left[i] : 0);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kOut; ++i) {
+        const int64_t p = p0 + S::p_piece(wave, i * kBy) / kBy * 16 + col;
+        if (!WHOLE && left[i] <= 0) continue;
         float bias[kBy][4], scale[kBy][4];
         if constexpr (FORM == kForward) {
 #pragma unroll
             for (int w = 0; w < kBy; ++w) {
+                Four<O> b;
+                Four<float> s;
+                b.v = decltype(b.v){};
+                if (a.bias[w]) b = load4<O, false>(reinterpret_cast<const O*>(a.bias[w]) + p, left[i]);
+                if constexpr (sizeof(T) == 1) s = load4<float, false>(a.p_scale[w] + p, left[i]);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) { bias[w][e] = 0.f; scale[w][e] = 1.f; }
-                if (a.bias[w]) load4(reinterpret_cast<const O*>(a.bias[w]) + p, n, false, bias[w]);
-                if constexpr (sizeof(T) == 1) load4(a.p_scale[w] + p, n, false, scale[w]);
+                for (int e = 0; e < 4; ++e) {
+                    bias[w][e] = to_float(b.e[e]);
+                    if constexpr (sizeof(T) == 1) scale[w][e] = s.e[e];
+                }
             }
         }
 #pragma unroll
         for (int j = 0; j < S::FQ; ++j) {
-            const int64_t q = q0 + S::q_piece(wave, j) * 16 + (lane & 15);
-            if (q >= a.q_count) continue;
+            const int64_t q = q0 + S::q_piece(wave, j) * 16 + row;
+            if (!WHOLE && q >= a.q_count) continue;
+            float o[4];
             if constexpr (FORM == kForward) {
                 float v[kBy][4];
                 const float qs = sizeof(T) == 1 ? a.q_scale[q] : 1.f;
@@ -99,53 +125,57 @@ __device__ __forceinline__ void epilogue(const Args& a, int64_t p0, int64_t q0, 
                 for (int w = 0; w < kBy; ++w)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        float t = acc[i + w][j][e];
+                        float t = acc[i * kBy + w][j][e];
                         if constexpr (sizeof(T) == 1) t *= qs * scale[w][e];
                         v[w][e] = t + bias[w][e];
                     }
-                float o[4];
                 if constexpr (GRAD) {
-                    float dy[4];
-                    load4(reinterpret_cast<const O*>(a.dy) + q * a.p_count + p, n, fours<O>(a.dy, a.p_count), dy);
-                    if constexpr (kPair) {
-                        float o2[4];
+                    float o2[4];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            o[e] = slope_of<EXACT>(a.act, v[0][e], dy[e] * v[1][e]);
-                            o2[e] = dy[e] * act_of<EXACT>(a.act, v[0][e]);
-                        }
-                        store4(reinterpret_cast<O*>(a.out[1]) + q * a.out_ld + p, n, vec_out, o2);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[e] = slope_of<EXACT>(a.act, v[0][e], dy[e]);
+                    for (int e = 0; e < 4; ++e) {
+                        const float dy = to_float(in[i][j].e[e]);
+                        o[e] = slope_of<EXACT, ACT>(v[0][e], kPair ? dy * v[kBy - 1][e] : dy);
+                        if constexpr (kPair) o2[e] = dy * act_of<EXACT, ACT>(v[0][e]);
                     }
+                    if constexpr (kPair) store4<O, WHOLE>(reinterpret_cast<O*>(a.out[1]) + q * a.out_ld + p, left[i], o2);
                 } else {
-                    if constexpr (kPair) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) o[e] = act_of<EXACT>(a.act, v[0][e]) * v[1][e];
-                    } else {
-                        float r[4] = {0.f, 0.f, 0.f, 0.f};
-                        if (a.residual) load4(reinterpret_cast<const O*>(a.residual) + q * a.p_count + p, n, fours<O>(a.residual, a.p_count), r);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[e] = act_of<EXACT>(a.act, v[0][e]) + r[e];
+                    for (int e = 0; e < 4; ++e) {
+                        o[e] = act_of<EXACT, ACT>(v[0][e]);
+                        if constexpr (kPair) o[e] *= v[1][e];
+                        else if (more) o[e] += to_float(in[i][j].e[e]);
                     }
                 }
-                store4(reinterpret_cast<O*>(a.out[0]) + q * a.out_ld + p, n, vec_out, o);
             } else {
-                const float o[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-                if (FORM == kWeightGrad && a.partial) {
-                    float* to = a.partial + ((int64_t)split * a.q_count + q) * a.p_count + p;
-                    store4(to, n, fours<float>(a.partial, a.p_count), o);
-                } else if (FORM == kWeightGrad && q >= a.q_first) {
-                    store4(reinterpret_cast<O*>(a.out[1]) + (q - a.q_first) * a.out_ld + p, n, vec_out, o);
-                } else {
-                    store4(reinterpret_cast<O*>(a.out[0]) + q * a.out_ld + p, n, vec_out, o);
-                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = acc[i][j][e];
             }
+            if (FORM == kWeightGrad && a.partial) store4<float, WHOLE>(a.partial + ((int64_t)split * a.q_count + q) * a.p_count + p, left[i], o);
+            else if (FORM == kWeightGrad && q >= a.q_first) store4<O, WHOLE>(reinterpret_cast<O*>(a.out[1]) + (q - a.q_first) * a.out_ld + p, left[i], o);
+            else store4<O, WHOLE>(reinterpret_cast<O*>(a.out[0]) + q * a.out_ld + p, left[i], o);
         }
     }
 }
-
+template <typename T, typename O, int FORM, bool TWO, bool GRAD, typename S>
+__device__ __forceinline__ void epilogue(const Args& a, int64_t p0, int64_t q0, unsigned split, const f32x4 (&acc)[S::FP][S::FQ]) {
+    constexpr int kCols = FORM == kForward && TWO ? S::kCols / 2 : S::kCols;
+    const void* more = GRAD ? a.dy : a.residual;
+    const bool whole = p0 + kCols <= a.p_count && q0 + S::kRows <= a.q_count &&
+                       (FORM == kWeightGrad && a.partial ? fours<float>(a.partial, a.p_count) : fours<O>(a.out[0], a.out_ld) && fours<O>(a.out[1], a.out_ld)) &&
+                       (!more || fours<O>(more, a.p_count));
+#define X(ACT) do { if (whole) finish<T, O, FORM, TWO, GRAD, S, ACT, true>(a, p0, q0, split, acc); else finish<T, O, FORM, TWO, GRAD, S, ACT, false>(a, p0, q0, split, acc); } while (0)
+    if constexpr (FORM != kForward) {
+        X(TGT_ACT_NONE);
+    } else {
+        switch (a.act) {
+            case TGT_ACT_SILU: X(TGT_ACT_SILU); break;
+            case TGT_ACT_GELU: X(TGT_ACT_GELU); break;
+            case TGT_ACT_RELU: X(TGT_ACT_RELU); break;
+            default: X(TGT_ACT_NONE); break;
+        }
+    }
+#undef X
+}
 
 template <typename T, typename O, int FORM, bool TWO, bool GRAD, bool ALIGNED, typename S, int STAGES>
 __global__ __launch_bounds__(S::kThreads) void k_product(const Args a) {
@@ -164,7 +194,7 @@ __global__ __launch_bounds__(S::kThreads) void k_product(const Args a) {
 template <typename T, typename O, int FORM, bool TWO, bool GRAD, typename S>
 __global__ __launch_bounds__(S::kThreads, 2) void k_wide(const Args a, const unsigned places, const unsigned splits) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    struct Place { int64_t p0, q0, steps; unsigned split; };
+    struct Place { int64_t p0, q0, k0, k1, steps; unsigned split; };
     Stream<T, FORM, TWO, S> stream;
     Place now, next;
     unsigned b = blockIdx.x;
@@ -175,9 +205,10 @@ __global__ __launch_bounds__(S::kThreads, 2) void k_wide(const Args a, const uns
             if (!tile_of(a, b % places, tp, tq)) continue;
             at.p0 = (int64_t)tp * (FORM == kForward && TWO ? S::kCols / 2 : S::kCols);
             at.q0 = (int64_t)tq * S::kRows;
-            const int64_t k0 = (int64_t)at.split * a.K_each, k1 = k0 + a.K_each < a.K ? k0 + a.K_each : a.K;
-            at.steps = (k1 - k0 + Kind<T>::kStep - 1) / Kind<T>::kStep;
-            stream.begin(a, at.p0, at.q0, k0, k1);
+            at.k0 = (int64_t)at.split * a.K_each;
+            at.k1 = at.k0 + a.K_each < a.K ? at.k0 + a.K_each : a.K;
+            at.steps = (at.k1 - at.k0) / Kind<T>::kStep;
+            stream.begin(a, at.p0, at.q0, at.k0);
             b += gridDim.x;
             return true;
         }
@@ -192,6 +223,8 @@ __global__ __launch_bounds__(S::kThreads, 2) void k_wide(const Args a, const uns
         asm volatile("" ::: "memory");
         f32x4 acc[S::FP][S::FQ];
         stream.product(now.steps, lds, acc);
+        const int64_t done = now.k0 + now.steps * Kind<T>::kStep;
+        if (done < now.k1) stream.rest(a, now.p0, now.q0, done, now.k1, lds, acc);
         more = find(next);
         if (more) stream.ask_first(lds, next.steps);
         epilogue<T, O, FORM, TWO, GRAD, S>(a, now.p0, now.q0, now.split, acc);
