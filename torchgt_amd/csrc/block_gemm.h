@@ -244,19 +244,22 @@ template <typename T, bool KC, int COUNT, int THREADS, bool ALIGNED> struct Tile
 namespace tgt {
 namespace gemm {
 
-// (the sum of one element once more, in plain multiply-adds: float32, where the parts' sum came out NaN)
-template <int FORM> __device__ __noinline__ float again(const Args& a, int which, int64_t q, int64_t p, int64_t k0, int64_t k1) {
-    const float* Q = reinterpret_cast<const float*>(a.Q);
-    const float* P = reinterpret_cast<const float*>(a.P[which]);
-    float s = 0.f;
-    for (int64_t k = k0; k < k1 && s == s; ++k) {
-        float y;
-        if (FORM == kForward) y = P[p * a.p_ld + k];
-        else if (FORM == kInputGrad) y = k < a.K_first ? P[k * a.p_ld + p] : reinterpret_cast<const float*>(a.P[1])[(k - a.K_first) * a.p_ld + p];
-        else y = P[k * a.p_ld + p];
-        s = __builtin_fmaf(FORM == kWeightGrad ? Q[k * a.q_ld + q] : Q[q * a.q_ld + k], y, s);
-    }
+// s + sum of x[k xs] y[k ys], in plain multiply-adds: where the parts' sum came out NaN.  (Its arguments are values: the address of the kernel's would put them, and
+// every pointer among them, into scratch memory.)
+static __device__ __noinline__ float again(float s, const float* x, int64_t xs, const float* y, int64_t ys, int64_t n) {
+    for (int64_t k = 0; k < n && s == s; ++k) s = __builtin_fmaf(x[k * xs], y[k * ys], s);
     return s;
+}
+template <int FORM> __device__ __forceinline__ float again(const Args& a, int which, int64_t q, int64_t p, int64_t k0, int64_t k1) {
+    const float* Q = reinterpret_cast<const float*>(a.Q) + (FORM == kWeightGrad ? k0 * a.q_ld + q : q * a.q_ld + k0);
+    const int64_t qs = FORM == kWeightGrad ? a.q_ld : 1;
+    const float* P = reinterpret_cast<const float*>(a.P[which]);
+    if (FORM == kForward) return again(0.f, Q, qs, P + p * a.p_ld + k0, 1, k1 - k0);
+    if (FORM == kInputGrad && k1 > a.K_first) {      // (k0 is 0)
+        const float s = again(0.f, Q, 1, P + p, a.p_ld, a.K_first);
+        return again(s, Q + a.K_first, 1, reinterpret_cast<const float*>(a.P[1]) + p, a.p_ld, k1 - a.K_first);
+    }
+    return again(0.f, Q, qs, P + k0 * a.p_ld + p, a.p_ld, k1 - k0);
 }
 
 // Tile shape: COLS x ROWS of the result by WP x WQ waves
@@ -377,11 +380,15 @@ __device__ __forceinline__ void product(const Args& a, int64_t p0, int64_t q0, i
     }
 }
 
-// Workgroup -> tile.  Consecutive workgroups go to the eight XCDs in turn, each with an L2 of its own: XCD x takes the tiles from x / 8 of
-// the way on, eight rows of tiles at a time, column by column, so that the tiles that run there together share both operands.
-__device__ __forceinline__ bool tile_of(const Args& a, unsigned b, unsigned& tp, unsigned& tq) {
-    const unsigned n = a.p_tiles * a.q_tiles, each = (n + 7) / 8, t = (b & 7) * each + (b >> 3);
+// Workgroup -> tile and split.  Consecutive workgroups go to the eight XCDs in turn, each with an L2 of its own: XCD x takes the places from x / 8 of
+// the way on; one split after the other, of a split eight rows of tiles at a time, column by column, so that the tiles that run there together
+// share both operands.
+__device__ __forceinline__ bool tile_of(const Args& a, unsigned splits, unsigned b, unsigned& tp, unsigned& tq, unsigned& split) {
+    const unsigned tiles = a.p_tiles * a.q_tiles, n = tiles * splits, each = (n + 7) / 8;
+    unsigned t = (b & 7) * each + (b >> 3);
     if ((b >> 3) >= each || t >= n) return false;
+    split = t / tiles;
+    t -= split * tiles;
     constexpr unsigned kBand = 8;
     const unsigned band = t / (kBand * a.p_tiles), rest = t - band * kBand * a.p_tiles;
     const unsigned high = min(kBand, a.q_tiles - band * kBand);

@@ -178,18 +178,18 @@ __device__ __forceinline__ void epilogue(const Args& a, int64_t p0, int64_t q0, 
 }
 
 template <typename T, typename O, int FORM, bool TWO, bool GRAD, bool ALIGNED, typename S, int STAGES>
-__global__ __launch_bounds__(S::kThreads) void k_product(const Args a) {
+__global__ __launch_bounds__(S::kThreads) void k_product(const Args a, const unsigned splits) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    unsigned tp, tq;
-    if (!tile_of(a, blockIdx.x, tp, tq)) return;
+    unsigned tp, tq, split;
+    if (!tile_of(a, splits, blockIdx.x, tp, tq, split)) return;
     const int64_t p0 = (int64_t)tp * (FORM == kForward && TWO ? S::kCols / 2 : S::kCols), q0 = (int64_t)tq * S::kRows;
-    const int64_t k0 = (int64_t)blockIdx.y * a.K_each, k1 = k0 + a.K_each < a.K ? k0 + a.K_each : a.K;
+    const int64_t k0 = (int64_t)split * a.K_each, k1 = k0 + a.K_each < a.K ? k0 + a.K_each : a.K;
     f32x4 acc[S::FP][S::FQ];
     product<T, FORM, TWO, ALIGNED, S, STAGES>(a, p0, q0, k0, k1, lds, acc);
-    epilogue<T, O, FORM, TWO, GRAD, S>(a, p0, q0, blockIdx.y, acc);
+    epilogue<T, O, FORM, TWO, GRAD, S>(a, p0, q0, split, acc);
 }
 
-// Large products: workgroup b takes the places b, b + gridDim.x, ... of the order of tiles (and splits); gridDim.x is a multiple of eight, so its
+// Large products: workgroup b takes the places b, b + gridDim.x, ... of tile_of's order; gridDim.x is a multiple of eight, so its
 // tiles stay on its XCD.  The next tile's first operands are asked for before this one's results are written.
 template <typename T, typename O, int FORM, bool TWO, bool GRAD, typename S>
 __global__ __launch_bounds__(S::kThreads, 2) void k_wide(const Args a, const unsigned places, const unsigned splits) {
@@ -199,10 +199,9 @@ __global__ __launch_bounds__(S::kThreads, 2) void k_wide(const Args a, const uns
     Place now, next;
     unsigned b = blockIdx.x;
     auto find = [&](Place& at) {      // the next place that has a tile, its operands' addresses
-        for (; b < places * splits; b += gridDim.x) {
+        for (; b < places; b += gridDim.x) {
             unsigned tp, tq;
-            at.split = b / places;
-            if (!tile_of(a, b % places, tp, tq)) continue;
+            if (!tile_of(a, splits, b, tp, tq, at.split)) continue;
             at.p0 = (int64_t)tp * (FORM == kForward && TWO ? S::kCols / 2 : S::kCols);
             at.q0 = (int64_t)tq * S::kRows;
             at.k0 = (int64_t)at.split * a.K_each;
@@ -229,6 +228,94 @@ __global__ __launch_bounds__(S::kThreads, 2) void k_wide(const Args a, const uns
         if (more) stream.ask_first(lds, next.steps);
         epilogue<T, O, FORM, TWO, GRAD, S>(a, now.p0, now.q0, now.split, acc);
     }
+}
+
+// Products of few rows (up to 16 NQ): bound by the weights' bytes.  A workgroup has 16 columns of the result, its waves a share of the contraction each, operands go
+// from memory to the matrix instructions without LDS, and the waves' sums are added in their order.  A wave asks for U steps of both operands at once;
+// with 16 waves that is 100 to 200 KB in flight on a CU.
+//   float32: v_mfma_f32_16x16x4_f32, products exact (a memory-bound kernel has no use for three parts)
+template <int BY, int NQ> struct FewShape {
+    static constexpr int kCols = 16 * BY, kRows = 16 * NQ, FP = BY, FQ = 1;
+    static __device__ __forceinline__ int p_piece(int, int i) { return i; }
+    static __device__ __forceinline__ int q_piece(int wave, int) { return wave; }
+};
+template <typename T, typename O, bool TWO, int NQ, bool ALIGNED>
+__global__ __launch_bounds__(1024) void k_few(const Args a) {
+    constexpr int BY = TWO ? 2 : 1, CE = 16 / (int)sizeof(T), U = NQ == 4 ? 2 : 4;
+    using S = FewShape<BY, NQ>;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, g = lane >> 4;
+    const int64_t p0 = (int64_t)blockIdx.x * 16;
+    const int64_t pr = p0 + (lane & 15) < a.p_count ? p0 + (lane & 15) : a.p_count - 1;
+    const T *W[BY], *X[NQ];
+#pragma unroll
+    for (int w = 0; w < BY; ++w) W[w] = reinterpret_cast<const T*>(a.P[w]) + pr * a.p_ld;
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) {
+        const int64_t q = 16 * j + (lane & 15) < a.q_count ? 16 * j + (lane & 15) : a.q_count - 1;
+        X[j] = reinterpret_cast<const T*>(a.Q) + q * a.q_ld;
+    }
+    constexpr int kAtOnce = 4 * CE * U;      // contraction indices that a wave asks for at once
+    const int64_t each = (a.K + (int64_t)waves * kAtOnce - 1) / ((int64_t)waves * kAtOnce) * kAtOnce;
+    const int64_t k0 = wave * each, k1 = k0 + each < a.K ? k0 + each : a.K;
+    f32x4 acc[BY][NQ];
+#pragma unroll
+    for (int w = 0; w < BY; ++w)
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) acc[w][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int64_t k = k0; k < k1; k += kAtOnce) {
+        u32x4 wv[BY][U], xv[NQ][U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t at = k + u * 4 * CE + g * CE;
+#pragma unroll
+            for (int w = 0; w < BY; ++w) wv[w][u] = part_of_row<T, ALIGNED>(W[w], at, k1, true);
+#pragma unroll
+            for (int j = 0; j < NQ; ++j) xv[j][u] = part_of_row<T, ALIGNED>(X[j], at, k1, true);
+        }
+#pragma unroll
+        for (int w = 0; w < BY; ++w)
+#pragma unroll
+            for (int j = 0; j < NQ; ++j) {
+                f32x4& c = acc[w][j];
+                if constexpr (sizeof(T) == 1) {
+#pragma unroll
+                    for (int u = 0; u < U; u += 2) {
+                        union { u32x4 h[2]; i32x8 v; } x, y;
+                        x.h[0] = wv[w][u]; x.h[1] = wv[w][u + 1];
+                        y.h[0] = xv[j][u]; y.h[1] = xv[j][u + 1];
+                        c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x.v, y.v, c, 0, 0, 0, 0, 0, 0);
+                    }
+                } else if constexpr (sizeof(T) == 2) {
+#pragma unroll
+                    for (int u = 0; u < U; ++u) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, wv[w][u]), __builtin_bit_cast(bf16x8, xv[j][u]), c, 0, 0, 0);
+                } else {
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(wv[w][u][e]), __uint_as_float(xv[j][u][e]), c, 0, 0, 0);
+                }
+            }
+    }
+    f32x4* sums = reinterpret_cast<f32x4*>(lds);      // [waves][BY][NQ][64]
+#pragma unroll
+    for (int w = 0; w < BY; ++w)
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) sums[((wave * BY + w) * NQ + j) * 64 + lane] = acc[w][j];
+    __syncthreads();
+    if (wave >= NQ) return;
+    f32x4 total[BY][1];
+#pragma unroll
+    for (int w = 0; w < BY; ++w) {
+        f32x4 t = sums[(w * NQ + wave) * 64 + lane];
+        for (int v = 1; v < waves; ++v) {
+            const f32x4 s = sums[((v * BY + w) * NQ + wave) * 64 + lane];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) t[e] += s[e];
+        }
+        total[w][0] = t;
+    }
+    epilogue<T, O, kForward, TWO, false, S>(a, p0, 0, 0, total);
 }
 
 #if TGT_GATED_PART == 0
@@ -270,7 +357,7 @@ int launch(Args a, int splits, hipStream_t st) {
     constexpr int kCols = FORM == kForward && TWO ? S::kCols / 2 : S::kCols;
     a.p_tiles = (unsigned)((a.p_count + kCols - 1) / kCols);
     a.q_tiles = (unsigned)((a.q_count + S::kRows - 1) / S::kRows);
-    const int64_t tiles = (int64_t)a.p_tiles * a.q_tiles;
+    const int64_t tiles = (int64_t)a.p_tiles * a.q_tiles * splits;
     if (tiles > (1ll << 30)) { set_error("torchgt: a product of more than 2^30 tiles"); return TGT_ERR_UNSUPPORTED; }
     constexpr int kLds = STAGES * (S::kCols + S::kRows) * Kind<T>::kRowBytes * Kind<T>::kPlanes;
     auto* kernel = k_product<T, O, FORM, TWO, GRAD, ALIGNED, S, STAGES>;
@@ -279,7 +366,7 @@ int launch(Args a, int splits, hipStream_t st) {
         const int rc = allow_lds((const void*)kernel, kLds, done);
         if (rc != TGT_OK) return rc;
     }
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((tiles + 7) / 8 * 8), (unsigned)splits), dim3(S::kThreads), kLds, st, a);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(S::kThreads), kLds, st, a, (unsigned)splits);
     TGT_HIP_CHECK(hipGetLastError());
     return TGT_OK;
 }
@@ -289,18 +376,33 @@ int launch_wide(Args a, int splits, hipStream_t st) {
     constexpr int kCols = FORM == kForward && TWO ? S::kCols / 2 : S::kCols;
     a.p_tiles = (unsigned)((a.p_count + kCols - 1) / kCols);
     a.q_tiles = (unsigned)((a.q_count + S::kRows - 1) / S::kRows);
-    const int64_t places = ((int64_t)a.p_tiles * a.q_tiles + 7) / 8 * 8;
-    if (places * splits > (1ll << 30)) { set_error("torchgt: a product of more than 2^30 tiles"); return TGT_ERR_UNSUPPORTED; }
+    const int64_t places = ((int64_t)a.p_tiles * a.q_tiles * splits + 7) / 8 * 8;
+    if (places > (1ll << 30)) { set_error("torchgt: a product of more than 2^30 tiles"); return TGT_ERR_UNSUPPORTED; }
     auto* kernel = k_wide<T, O, FORM, TWO, GRAD, S>;
     static std::atomic<uint64_t> done{0};
     const int rc = allow_lds((const void*)kernel, S::kLds, done);
     if (rc != TGT_OK) return rc;
-    const unsigned grid = (unsigned)std::min<int64_t>(places * splits, num_cus() / 8 * 8);
+    const unsigned grid = (unsigned)std::min<int64_t>(places, num_cus() / 8 * 8);
     hipLaunchKernelGGL(kernel, dim3(grid), dim3(S::kThreads), S::kLds, st, a, (unsigned)places, (unsigned)splits);
     TGT_HIP_CHECK(hipGetLastError());
     return TGT_OK;
 }
 
+template <typename T, typename O, bool TWO, int NQ, bool ALIGNED> int launch_few(const Args& a, hipStream_t st) {
+    constexpr int kBy = TWO ? 2 : 1, kAtOnce = 4 * (16 / (int)sizeof(T)) * (NQ == 4 ? 2 : 4);
+    // a share of the contraction for each wave, 4 (16 rows for each: so many lanes that add up) to 16 waves
+    const int waves = (int)std::max<int64_t>(4, std::min<int64_t>(16, (a.K + kAtOnce - 1) / kAtOnce));
+    const int bytes = waves * kBy * NQ * 64 * 16;      // at most 128 KB
+    auto* kernel = k_few<T, O, TWO, NQ, ALIGNED>;
+    if (16 * kBy * NQ * 64 * 16 > 65536) {
+        static std::atomic<uint64_t> done{0};
+        const int rc = allow_lds((const void*)kernel, 16 * kBy * NQ * 64 * 16, done);
+        if (rc != TGT_OK) return rc;
+    }
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((a.p_count + 15) / 16)), dim3(64 * waves), bytes, st, a);
+    TGT_HIP_CHECK(hipGetLastError());
+    return TGT_OK;
+}
 // Tiles of `cols` x 256 that keep the CUs busy
 bool wide_enough(const Args& a, int cols, int splits) {
     const int64_t tiles = (a.p_count + cols - 1) / cols * ((a.q_count + 255) / 256) * splits;
@@ -321,6 +423,12 @@ template <typename T, typename O> int product_forward(const Args& a, bool grad, 
     constexpr int kStages = sizeof(T) == 4 ? 1 : 2;
     const bool two = a.P[1] != nullptr;
     const bool al = aligned16(a.Q, a.q_ld, sizeof(T)) && aligned16(a.P[0], a.p_ld, sizeof(T)) && (!two || aligned16(a.P[1], a.p_ld, sizeof(T)));
+    if (!grad && a.q_count <= 64) {
+#define X(TWO, NQ, AL) if (two == TWO && a.q_count <= 16 * NQ && al == AL) return launch_few<T, O, TWO, NQ, AL>(a, st)
+        X(false, 1, true); X(true, 1, true); X(false, 2, true); X(true, 2, true); X(false, 4, true); X(true, 4, true);
+        X(false, 1, false); X(true, 1, false); X(false, 2, false); X(true, 2, false); X(false, 4, false); X(true, 4, false);
+#undef X
+    }
     if constexpr (sizeof(T) < 4) {
         if (al && wide_enough(a, two ? 128 : 256, 1)) {
 #define X(TWO, GRAD) if (two == TWO && grad == GRAD) return launch_wide<T, O, kForward, TWO, GRAD, Wide<2>>(a, 1, st)
@@ -536,7 +644,14 @@ int backward(const Call& c, const void* dy, void* dx, void* const* dW, void* con
         KernelTimer t(KS_LINEAR_DW, st);
         rc = f32 ? product_weight_grad<float>(a, p.splits, st) : product_weight_grad<b16>(a, p.splits, st);
         if (rc != TGT_OK) return rc;
-        if (p.splits > 1) {
+        if (p.splits >= 8 && cols * c.K < (1 << 30)) {      // few elements, many splits: 16 slices of the splits side by side
+            tgt_reduce_desc r{};
+            r.partial = a.partial; r.workers = p.splits; r.n = (int)(cols * c.K); r.n_out = c.n;
+            r.out[0] = dW[0];
+            if (c.n == 2) { r.out[1] = dW[1]; r.begin[1] = c.F * c.K; }
+            rc = reduce_partials(&r, 1, c.dtype, st);
+            if (rc != TGT_OK) return rc;
+        } else if (p.splits > 1) {
             const int64_t n = cols * c.K, first = (int64_t)c.F * c.K;
             const dim3 grid((unsigned)((n + 255) / 256));
             if (f32) hipLaunchKernelGGL((k_add_splits<float>), grid, dim3(256), 0, st, a.partial, p.splits, n, first, (float*)dW[0], (float*)a.out[1]);
