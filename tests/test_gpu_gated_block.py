@@ -198,6 +198,30 @@ def test_gated_linear_gradient_is_that_of_differences(cuda):
         near(outs[k], want, torch.full_like(want, 1e-5 * float(want.abs().max())), k)
 
 
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("rows", [40, 400])
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+def test_activations_of_any_argument(cuda, act, dt, rows):
+    """One feature, weight one: values and slopes over the whole range, kernels for few rows and for many.  float32: 2^-20 of 1 + |u|, what a few units in the last
+    place of exp and a distribution function near one may cost; bfloat16 half a step more."""
+    g = torch.Generator().manual_seed(2)
+    big = torch.tensor([0.0, -0.0, 1e-30, -1e-30, 5.0, -5.0, 20.0, -20.0, 60.0, -60.0, 88.0, -88.0, 104.0, -104.0, 1e4, -1e4, 1e30, -1e30])
+    x = torch.cat([big, rand(g, rows - len(big), scale=3, device="cpu")]).to(dt).cuda()[:, None]
+    one = torch.ones(1, 1, device="cuda", dtype=dt)
+    xl = x.clone().requires_grad_(True)
+    y = T.linear_act(xl, one, activation=act)
+    (gx,) = torch.autograd.grad(y, xl, torch.ones_like(y))
+    u = d(x)
+    want = act64(act, u)
+    near(y, want, half_step(dt) * want.abs() + fine(dt) * torch.minimum(1 + u.abs(), 1 + want.abs()), "value")
+    s = slope64(act, u).nan_to_num(0)
+    near(gx, s, 2 * half_step(dt) * s.abs() + fine(dt) * 4, "slope")
+    with torch.no_grad():
+        near(T.linear_act(x, one, activation=act), want, half_step(dt) * want.abs() + fine(dt) * torch.minimum(1 + u.abs(), 1 + want.abs()), "value")
+        h = T.gated_linear(x, one, 0 * one, up_bias=one[0], activation=act)      # act(u) * 1
+        near(h, want, half_step(dt) * want.abs() + fine(dt) * torch.minimum(1 + u.abs(), 1 + want.abs()), "gated")
+
+
 def test_only_some_gradients_wanted(cuda):
     x, wg, wu, bg, bu, dh = gated_case(50, 32, 48, F32, "silu", True)
     full = run_gated(x, wg, wu, bg, bu, dh, "silu")

@@ -10,34 +10,15 @@
 // the tensors' type, since they are operands of the next two products; that costs as much as the rounding of any other activation).  Keeping
 // them would cost 4 F values of memory per node and their rounding would go into act'.  dx and dW are products of what it wrote.
 // dW over few output tiles is cut along the nodes, partial sums in float32 added in a fixed order.
+#include "activations.h"
 #include "block_gemm.h"
+#include "gated_tiles.h"
 #include <algorithm>
 
 namespace tgt {
 namespace {
 
 using namespace gemm;
-
-// act(u), and dh * act'(u).  SILU: u / (1 + exp(-u)); EXACT (float32 results): with expf and a division, else with the hardware's exp2 and reciprocal, which are
-// good to 2^-22 and 2^-14 |u| of a result of 8 bits
-template <bool EXACT> __device__ __forceinline__ float sigmoid_of(float u) {
-    return EXACT ? 1.f / (1.f + expf(-u)) : __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(u * -1.4426950408889634f));
-}
-template <bool EXACT, int ACT> __device__ __forceinline__ float act_of(float u) {
-    if (ACT == TGT_ACT_SILU) return EXACT ? u / (1.f + expf(-u)) : u * sigmoid_of<false>(u);
-    if (ACT == TGT_ACT_GELU) return act_value<false>(u);
-    if (ACT == TGT_ACT_RELU) return act_value<true>(u);
-    return u;
-}
-template <bool EXACT, int ACT> __device__ __forceinline__ float slope_of(float u, float dh) {
-    if (ACT == TGT_ACT_SILU) {
-        const float s = sigmoid_of<EXACT>(u);
-        return dh * (s * (1.f + u * (1.f - s)));
-    }
-    if (ACT == TGT_ACT_GELU) return act_grad<false>(u, dh);
-    if (ACT == TGT_ACT_RELU) return act_grad<true>(u, dh);
-    return dh;
-}
 
 // Four neighbouring elements of a row in memory
 template <typename O> struct Four { O e[4]; };
@@ -319,30 +300,55 @@ __global__ __launch_bounds__(1024) void k_few(const Args a) {
 }
 
 #if TGT_GATED_PART == 0
-// Sums over the splits of a weight gradient, in their order.  Elements from q_first rows on go to the second output.
+// Sums over the splits of a weight gradient, in their order, four elements a thread.  Elements from n_first on go to the second output.
 template <typename O> __global__ __launch_bounds__(256) void k_add_splits(const float* __restrict__ partial, int splits, int64_t n, int64_t n_first, O* __restrict__ out0,
                                                                           O* __restrict__ out1) {
-    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
     if (e >= n) return;
-    float s = 0.f;
-    for (int w = 0; w < splits; ++w) s += partial[w * n + e];
-    O v;
-    from_float(v, s);
-    if (e < n_first) out0[e] = v;
-    else out1[e - n_first] = v;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    if (n % 4 == 0) {
+#pragma unroll 4
+        for (int w = 0; w < splits; ++w) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(partial + w * n + e);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[i] += v[i];
+        }
+    } else {
+        for (int w = 0; w < splits; ++w)
+            for (int i = 0; i < 4; ++i)
+                if (e + i < n) s[i] += partial[w * n + e + i];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (e + i < n) from_float(e + i < n_first ? out0[e + i] : out1[e + i - n_first], s[i]);
 }
 
-// Column sums of a matrix of rows of M elements: workgroup (columns, share of the rows) -> partial[share][M]
+// Column sums of a matrix of rows of M elements: workgroup (64 columns, share of the rows) -> partial[share][M].  Eight rows in flight a wave; bound by their
+// latency where there are few columns.
 template <typename O> __global__ __launch_bounds__(256) void k_column_sums(const O* __restrict__ x, int64_t N, int64_t M, int64_t rows_each, float* __restrict__ partial) {
     __shared__ float part[4][64];
     const int c = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int64_t col = (int64_t)blockIdx.x * 64 + c, r0 = blockIdx.y * rows_each, r1 = r0 + rows_each < N ? r0 + rows_each : N;
     float s = 0.f;
-    if (col < M)
-        for (int64_t r = r0 + w; r < r1; r += 4) s += to_float(x[r * M + col]);
+    if (col < M) {
+        int64_t r = r0 + w;
+        for (; r + 28 < r1; r += 32) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = to_float(x[(r + 4 * i) * M + col]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s += v[i];
+        }
+        for (; r < r1; r += 4) s += to_float(x[r * M + col]);
+    }
     part[w][c] = s;
     __syncthreads();
     if (w == 0 && col < M) partial[blockIdx.y * M + col] = (part[0][c] + part[1][c]) + (part[2][c] + part[3][c]);
+}
+
+// Rows F .. Fp - 1 of a weight are zeros
+template <typename O> __global__ __launch_bounds__(256) void k_pad_rows(const O* __restrict__ w, int64_t n, int64_t all, O* __restrict__ out) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) out[i] = i < n ? w[i] : O{};
 }
 
 __global__ __launch_bounds__(256) void k_zero(uint16_t* __restrict__ p, int64_t n) {
@@ -530,10 +536,36 @@ Args forward_args(const Call& c) {
     return a;
 }
 
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+int in16(int dtype) { return dtype == TGT_DTYPE_F32 ? 4 : 8; }      // elements in 16 bytes
+// Whether the kernels for small widths (gated_tiles.hip, linear_tiles.hip) are the faster ones: weights of up to a million values and, forward + backward in us,
+// those kernels / the tiles of 128 and 256:   float32   300 x 128 x 128 25 / 59    2000 x 1024 x 1024 166 / 275   64000 x 256 x 256 206 / 236
+//                                                       64000 x 512 x 512 868 / 800      16000 x 1024 x 1024 827 / 756
+//                                             bfloat16  2000 x 512 x 512 47 / 59       16000 x 256 x 512 60 / 72         64000 x 256 x 256 94 / 101
+//                                                       64000 x 512 x 512 307 / 187      16000 x 1024 x 1024 316 / 174
+bool narrow(const Call& c) {
+    const double products = (double)c.N * c.K * c.F * c.n;
+    return (int64_t)c.K * c.F * c.n <= (1 << 20) && products <= (c.dtype == TGT_DTYPE_F32 ? 8.6e9 : 2.1e9) && c.K % in16(c.dtype) == 0 && aligned16(c.x) &&
+           aligned16(c.W[0]) && aligned16(c.W[1]);
+}
+NarrowArgs narrow_args(const Call& c, const void* more) {
+    NarrowArgs a{};
+    a.x = c.x; a.more = more;
+    for (int w = 0; w < c.n; ++w) { a.W[w] = c.W[w]; a.bias[w] = c.b[w]; }
+    a.N = c.N; a.K = c.K; a.F = a.out_ld = c.F; a.act = c.act;
+    return a;
+}
+
 int forward(const Call& c, const void* residual, void* out, hipStream_t st) {
     int rc = check_call(c);
     if (rc != TGT_OK || c.N == 0) return rc;
     if (!out) { set_error("%s: null pointer", c.who); return TGT_ERR_INVALID_ARG; }
+    if (c.N > 64 && narrow(c)) {
+        NarrowArgs a = narrow_args(c, residual);
+        a.out[0] = out;
+        KernelTimer t(KS_LINEAR_FWD, st);
+        return gated_tiles(a, false, c.dtype, st);
+    }
     Args a = forward_args(c);
     a.residual = residual;
     a.out[0] = out;
@@ -581,6 +613,60 @@ Plan plan_of(int n, int64_t N, int K, int F, int dtype, int act) {
     return p;
 }
 
+int64_t workspace_bytes_of(int n, int64_t N, int K, int F, int dtype, int act);
+
+// The backward where the widths are small: one kernel for dg and du, rows of 16 bytes, then the linears' own backward of two weights of one shape (which reads them
+// once for dx and once for all weight and bias gradients)
+int padded_width(int F, int dtype) { return (F + in16(dtype) - 1) / in16(dtype) * in16(dtype); }
+bool needs_du(int n, int act) { return n == 2 || act != TGT_ACT_NONE; }
+int64_t narrow_bytes(int n, int64_t N, int K, int F, int dtype, int act) {
+    const int64_t Fp = padded_width(F, dtype), size = dtype == TGT_DTYPE_F32 ? 4 : 2;
+    return (needs_du(n, act) ? n * up16(N * Fp * size) : 0) + (Fp != F ? up16(Fp * K * size) : 0) + up16(tgt_linear_bwd_workspace_bytes(n, K, (int)Fp));
+}
+int backward_narrow(const Call& c, const void* dy, void* dx, void* const* dW, void* const* db, char* ws, hipStream_t st) {
+    const int Fp = padded_width(c.F, c.dtype);
+    const bool f32 = c.dtype == TGT_DTYPE_F32;
+    const int64_t size = f32 ? 4 : 2;
+    const void *du[2] = {dy, nullptr}, *W[2] = {c.W[0], c.W[1]};
+    if (needs_du(c.n, c.act)) {
+        NarrowArgs a = narrow_args(c, dy);
+        for (int w = 0; w < c.n; ++w) { du[w] = a.out[w] = ws; ws += up16(c.N * Fp * size); }
+        a.out_ld = Fp;
+        KernelTimer t(KS_LINEAR_FWD, st);
+        if (const int rc = gated_tiles(a, true, c.dtype, st)) return rc;
+    }
+    if (Fp != c.F) {      // (one weight: its rows behind the last are zeros for dx, their gradients are not wanted)
+        const int64_t n = (int64_t)c.F * c.K, all = (int64_t)Fp * c.K;
+        const dim3 grid((unsigned)std::min<int64_t>((all + 255) / 256, 1024));
+        if (f32) hipLaunchKernelGGL((k_pad_rows<float>), grid, dim3(256), 0, st, (const float*)c.W[0], n, all, (float*)ws);
+        else hipLaunchKernelGGL((k_pad_rows<b16>), grid, dim3(256), 0, st, (const b16*)c.W[0], n, all, (b16*)ws);
+        TGT_HIP_CHECK(hipGetLastError());
+        W[0] = ws;
+        ws += up16(all * size);
+    }
+    const bool want_w = dW && dW[0], want_b = db && (db[0] || (c.n == 2 && db[1]));
+    const int64_t bytes = tgt_linear_bwd_workspace_bytes(c.n, c.K, Fp);
+    if (!want_w && !want_b) return dx ? tgt_linear_bwd(c.x, W, du, c.n, c.N, c.K, Fp, c.dtype, dx, nullptr, nullptr, nullptr, 0, st) : TGT_OK;
+    tgt_reduce_desc r{};
+    void* any[2] = {ws, ws};      // (where the sums go is said below)
+    const int rc = tgt_linear_bwd_deferred(c.x, W, du, c.n, c.N, c.K, Fp, c.dtype, dx, any, any, ws, bytes, st, &r);
+    if (rc != TGT_OK) return rc;
+    const int each = Fp * c.K + Fp;
+    r.n_out = 0;
+    for (int w = 0; w < c.n; ++w) {
+        const auto put = [&](void* out, int begin) { r.out[r.n_out] = out; r.begin[r.n_out++] = w * each + begin; };
+        put(want_w ? dW[w] : nullptr, 0);
+        if (Fp != c.F) put(nullptr, c.F * c.K);
+        put(want_b ? db[w] : nullptr, Fp * c.K);
+        if (Fp != c.F) put(nullptr, Fp * c.K + c.F);
+    }
+    return reduce_partials(&r, 1, c.dtype, st);
+}
+// Two weights of odd widths would need their rows padded too, and a gradient of odd rows that is the operand itself cannot be: those go the general way
+bool narrow_backward(const Call& c, const void* dy) {
+    return narrow(c) && (padded_width(c.F, c.dtype) == c.F || (c.n == 1 && c.act != TGT_ACT_NONE)) && (needs_du(c.n, c.act) || aligned16(dy));
+}
+
 int backward(const Call& c, const void* dy, void* dx, void* const* dW, void* const* db, void* workspace, int64_t workspace_bytes, hipStream_t st) {
     int rc = check_call(c);
     if (rc != TGT_OK) return rc;
@@ -599,11 +685,13 @@ int backward(const Call& c, const void* dy, void* dx, void* const* dW, void* con
     }
     if (!dy) { set_error("%s: null pointer", c.who); return TGT_ERR_INVALID_ARG; }
     const Plan p = plan_of(c.n, c.N, c.K, c.F, c.dtype, c.act);
-    if (!workspace || workspace_bytes < p.bytes || ((uintptr_t)workspace & 15)) {
-        set_error("%s: workspace of %lld bytes (16-byte aligned) needed, got %lld", c.who, (long long)p.bytes, (long long)workspace_bytes);
+    const int64_t need = workspace_bytes_of(c.n, c.N, c.K, c.F, c.dtype, c.act);
+    if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)) {
+        set_error("%s: workspace of %lld bytes (16-byte aligned) needed, got %lld", c.who, (long long)need, (long long)workspace_bytes);
         return TGT_ERR_WORKSPACE;
     }
     char* ws = (char*)workspace;
+    if (narrow_backward(c, dy)) return backward_narrow(c, dy, dx, dW, db, ws, st);
     const void* du = dy;
     if (p.du_bytes) {
         Args a = forward_args(c);
@@ -644,7 +732,7 @@ int backward(const Call& c, const void* dy, void* dx, void* const* dW, void* con
         KernelTimer t(KS_LINEAR_DW, st);
         rc = f32 ? product_weight_grad<float>(a, p.splits, st) : product_weight_grad<b16>(a, p.splits, st);
         if (rc != TGT_OK) return rc;
-        if (p.splits >= 8 && cols * c.K < (1 << 30)) {      // few elements, many splits: 16 slices of the splits side by side
+        if (p.splits >= 16 && cols * c.K <= 65536) {      // few elements, many splits: 16 slices of the splits side by side
             tgt_reduce_desc r{};
             r.partial = a.partial; r.workers = p.splits; r.n = (int)(cols * c.K); r.n_out = c.n;
             r.out[0] = dW[0];
@@ -653,7 +741,7 @@ int backward(const Call& c, const void* dy, void* dx, void* const* dW, void* con
             if (rc != TGT_OK) return rc;
         } else if (p.splits > 1) {
             const int64_t n = cols * c.K, first = (int64_t)c.F * c.K;
-            const dim3 grid((unsigned)((n + 255) / 256));
+            const dim3 grid((unsigned)((n + 1023) / 1024));
             if (f32) hipLaunchKernelGGL((k_add_splits<float>), grid, dim3(256), 0, st, a.partial, p.splits, n, first, (float*)dW[0], (float*)a.out[1]);
             else hipLaunchKernelGGL((k_add_splits<b16>), grid, dim3(256), 0, st, a.partial, p.splits, n, first, (b16*)dW[0], (b16*)a.out[1]);
             TGT_HIP_CHECK(hipGetLastError());
@@ -676,7 +764,11 @@ int backward(const Call& c, const void* dy, void* dx, void* const* dW, void* con
 
 int64_t workspace_bytes_of(int n, int64_t N, int K, int F, int dtype, int act) {
     if (N < 0 || K < 1 || F < 1 || (dtype != TGT_DTYPE_F32 && dtype != TGT_DTYPE_BF16)) return -1;
-    return N == 0 ? 0 : plan_of(n, N, K, F, dtype, act).bytes;
+    if (N == 0) return 0;
+    // (what decides which way a call goes is in part where its tensors lie: room for either)
+    const Call c{"", nullptr, {nullptr, nullptr}, {nullptr, nullptr}, n, N, K, F, dtype, act};
+    const int64_t general = plan_of(n, N, K, F, dtype, act).bytes;
+    return narrow(c) ? std::max(general, narrow_bytes(n, N, K, F, dtype, act)) : general;
 }
 
 }  // namespace
