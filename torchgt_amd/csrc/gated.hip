@@ -47,17 +47,31 @@ template <typename O, bool WHOLE> __device__ __forceinline__ void store4(O* p, i
             if (i < n) p[i] = f.e[i];
     }
 }
-template <typename O> __device__ __forceinline__ bool fours(const void* p, int64_t ld) { return ((uintptr_t)p & (4 * sizeof(O) - 1)) == 0 && (ld & 3) == 0; }
+template <typename O> __device__ __forceinline__ bool sixteens(const void* p, int64_t ld) { return ((uintptr_t)p & 15) == 0 && ld * sizeof(O) % 16 == 0; }
 
-// What becomes of a tile's sums.  WHOLE: the tile lies inside the result and all rows are aligned to four elements; what is read is then asked for
-// before the first value is formed.
+// Four columns of two neighbouring pieces of 16 become eight columns of one: lanes of the first and third 16 then have the first piece, the others the second
+// (and back: the exchange is its own inverse)
+__device__ __forceinline__ void exchange(uint2& first, uint2& second) {
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    const u32x2 x = __builtin_amdgcn_permlane16_swap(first.x, second.x, false, false), y = __builtin_amdgcn_permlane16_swap(first.y, second.y, false, false);
+    first = make_uint2(x[0], y[0]);
+    second = make_uint2(x[1], y[1]);
+}
+
+// What becomes of a tile's sums.  WHOLE: the tile lies inside the result and all rows are aligned to 16 bytes; what is read is then asked for before the
+// first value is formed, and 16-bit rows are read and written 16 bytes a lane, 64 in a row, by an exchange between the pieces (8 bytes a lane: 16 rows of 32 bytes an
+// instruction).
 template <typename T, typename O, int FORM, bool TWO, bool GRAD, typename S, int ACT, bool WHOLE>
 __device__ __forceinline__ void finish(const Args& a, int64_t p0, int64_t q0, unsigned split, const f32x4 (&acc)[S::FP][S::FQ]) {
     constexpr bool kPair = FORM == kForward && TWO, EXACT = sizeof(O) == 4, kReads = FORM == kForward && (GRAD || !TWO);
     constexpr int kBy = kPair ? 2 : 1, kOut = S::FP / kBy;      // pieces that one output piece takes
+    constexpr bool kWide = WHOLE && sizeof(O) == 2 && kOut % 2 == 0;
+    constexpr int kGroup = kWide ? 2 : 1;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = (lane >> 4) * 4, row = lane & 15;
+    const int wide_col = ((lane >> 4) & 1) * 16 + (lane >> 5) * 8;      // of 32
     const O* more = reinterpret_cast<const O*>(GRAD ? a.dy : a.residual);
+    const bool to_partial = FORM == kWeightGrad && a.partial;
     int left[kOut];
 #pragma unroll
     for (int i = 0; i < kOut; ++i) {
@@ -69,28 +83,37 @@ __device__ __forceinline__ void finish(const Args& a, int64_t p0, int64_t q0, un
 #pragma unroll
         for (int j = 0; j < S::FQ; ++j) {
             const int64_t q = q0 + S::q_piece(wave, j) * 16 + row;
-            const O* from = more + q * a.p_count + p0 + col;
+            const O* from = more + q * a.p_count + p0;
 #pragma unroll
-            for (int i = 0; i < kOut; ++i) in[kReads ? i : 0][j] = load4<O, WHOLE>(from + S::p_piece(wave, i * kBy) / kBy * 16, q < a.q_count ? left[i] : 0);
+            for (int i = 0; i < kOut; i += kGroup) {
+                const O* at = from + S::p_piece(wave, i * kBy) / kBy * 16;
+                if constexpr (kWide && kReads) {
+                    const u32x4 v = *reinterpret_cast<const u32x4*>(at + wide_col);
+                    in[i][j].v = make_uint2(v.x, v.y);
+                    in[i + 1][j].v = make_uint2(v.z, v.w);
+                } else in[kReads ? i : 0][j] = load4<O, WHOLE>(at + col, q < a.q_count ? left[i] : 0);
+            }
         }
     }
 #pragma unroll
-    for (int i = 0; i < kOut; ++i) {
-        const int64_t p = p0 + S::p_piece(wave, i * kBy) / kBy * 16 + col;
-        if (!WHOLE && left[i] <= 0) continue;
-        float bias[kBy][4], scale[kBy][4];
+    for (int i0 = 0; i0 < kOut; i0 += kGroup) {
+        float bias[kGroup][kBy][4], scale[kGroup][kBy][4];
         if constexpr (FORM == kForward) {
 #pragma unroll
-            for (int w = 0; w < kBy; ++w) {
-                Four<O> b;
-                Four<float> s;
-                b.v = decltype(b.v){};
-                if (a.bias[w]) b = load4<O, false>(reinterpret_cast<const O*>(a.bias[w]) + p, left[i]);
-                if constexpr (sizeof(T) == 1) s = load4<float, false>(a.p_scale[w] + p, left[i]);
+            for (int n = 0; n < kGroup; ++n) {
+                const int64_t p = p0 + S::p_piece(wave, (i0 + n) * kBy) / kBy * 16 + col;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    bias[w][e] = to_float(b.e[e]);
-                    if constexpr (sizeof(T) == 1) scale[w][e] = s.e[e];
+                for (int w = 0; w < kBy; ++w) {
+                    Four<O> b;
+                    Four<float> s;
+                    b.v = decltype(b.v){};
+                    if (a.bias[w]) b = load4<O, false>(reinterpret_cast<const O*>(a.bias[w]) + p, left[i0 + n]);
+                    if constexpr (sizeof(T) == 1) s = load4<float, false>(a.p_scale[w] + p, left[i0 + n]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        bias[n][w][e] = to_float(b.e[e]);
+                        if constexpr (sizeof(T) == 1) scale[n][w][e] = s.e[e];
+                    }
                 }
             }
         }
@@ -98,42 +121,67 @@ __device__ __forceinline__ void finish(const Args& a, int64_t p0, int64_t q0, un
         for (int j = 0; j < S::FQ; ++j) {
             const int64_t q = q0 + S::q_piece(wave, j) * 16 + row;
             if (!WHOLE && q >= a.q_count) continue;
-            float o[4];
-            if constexpr (FORM == kForward) {
-                float v[kBy][4];
-                const float qs = sizeof(T) == 1 ? a.q_scale[q] : 1.f;
+            if constexpr (kWide && kReads) {
+                if (more) exchange(in[i0][j].v, in[i0 + 1][j].v);
+            }
+            float o[kGroup][4], o2[kGroup][4];
 #pragma unroll
-                for (int w = 0; w < kBy; ++w)
+            for (int n = 0; n < kGroup; ++n) {
+                const int i = i0 + n;
+                if constexpr (FORM == kForward) {
+                    float v[kBy][4];
+                    const float qs = sizeof(T) == 1 ? a.q_scale[q] : 1.f;
+#pragma unroll
+                    for (int w = 0; w < kBy; ++w)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float t = acc[i * kBy + w][j][e];
+                            if constexpr (sizeof(T) == 1) t *= qs * scale[n][w][e];
+                            v[w][e] = t + bias[n][w][e];
+                        }
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        float t = acc[i * kBy + w][j][e];
-                        if constexpr (sizeof(T) == 1) t *= qs * scale[w][e];
-                        v[w][e] = t + bias[w][e];
+                        if constexpr (GRAD && kPair) {
+                            const float dy = to_float(in[i][j].e[e]);
+                            float f, s;
+                            act_and_slope<EXACT, ACT>(v[0][e], f, s);
+                            o[n][e] = dy * v[kBy - 1][e] * s;
+                            o2[n][e] = dy * f;
+                        } else if constexpr (GRAD) {
+                            o[n][e] = slope_of<EXACT, ACT>(v[0][e], to_float(in[i][j].e[e]));
+                        } else {
+                            o[n][e] = act_of<EXACT, ACT>(v[0][e]);
+                            if constexpr (kPair) o[n][e] *= v[1][e];
+                            else if (more) o[n][e] += to_float(in[i][j].e[e]);
+                        }
                     }
-                if constexpr (GRAD) {
-                    float o2[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float dy = to_float(in[i][j].e[e]);
-                        o[e] = slope_of<EXACT, ACT>(v[0][e], kPair ? dy * v[kBy - 1][e] : dy);
-                        if constexpr (kPair) o2[e] = dy * act_of<EXACT, ACT>(v[0][e]);
-                    }
-                    if constexpr (kPair) store4<O, WHOLE>(reinterpret_cast<O*>(a.out[1]) + q * a.out_ld + p, left[i], o2);
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        o[e] = act_of<EXACT, ACT>(v[0][e]);
-                        if constexpr (kPair) o[e] *= v[1][e];
-                        else if (more) o[e] += to_float(in[i][j].e[e]);
-                    }
+                    for (int e = 0; e < 4; ++e) o[n][e] = acc[i][j][e];
                 }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = acc[i][j][e];
             }
-            if (FORM == kWeightGrad && a.partial) store4<float, WHOLE>(a.partial + ((int64_t)split * a.q_count + q) * a.p_count + p, left[i], o);
-            else if (FORM == kWeightGrad && q >= a.q_first) store4<O, WHOLE>(reinterpret_cast<O*>(a.out[1]) + (q - a.q_first) * a.out_ld + p, left[i], o);
-            else store4<O, WHOLE>(reinterpret_cast<O*>(a.out[0]) + q * a.out_ld + p, left[i], o);
+            const int64_t p = p0 + S::p_piece(wave, i0 * kBy) / kBy * 16;
+            const auto put = [&](O* out, const float (&v)[kGroup][4]) {
+                if constexpr (kWide) {
+                    Four<O> f[2];
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) from_float(f[n].e[e], v[kGroup - 2 + n][e]);
+                    exchange(f[0].v, f[1].v);
+                    *reinterpret_cast<u32x4*>(out + wide_col) = u32x4{f[0].v.x, f[0].v.y, f[1].v.x, f[1].v.y};
+                } else store4<O, WHOLE>(out + col, left[i0], v[0]);
+            };
+            if (to_partial) {
+                float* out = a.partial + ((int64_t)split * a.q_count + q) * a.p_count + p + col;
+#pragma unroll
+                for (int n = 0; n < kGroup; ++n) store4<float, WHOLE>(out + 16 * n, left[i0 + n], o[n]);
+            } else if (FORM == kWeightGrad && q >= a.q_first) {
+                put(reinterpret_cast<O*>(a.out[1]) + (q - a.q_first) * a.out_ld + p, o);
+            } else {
+                put(reinterpret_cast<O*>(a.out[0]) + q * a.out_ld + p, o);
+                if constexpr (GRAD && kPair) put(reinterpret_cast<O*>(a.out[1]) + q * a.out_ld + p, o2);
+            }
         }
     }
 }
@@ -142,8 +190,8 @@ __device__ __forceinline__ void epilogue(const Args& a, int64_t p0, int64_t q0, 
     constexpr int kCols = FORM == kForward && TWO ? S::kCols / 2 : S::kCols;
     const void* more = GRAD ? a.dy : a.residual;
     const bool whole = p0 + kCols <= a.p_count && q0 + S::kRows <= a.q_count &&
-                       (FORM == kWeightGrad && a.partial ? fours<float>(a.partial, a.p_count) : fours<O>(a.out[0], a.out_ld) && fours<O>(a.out[1], a.out_ld)) &&
-                       (!more || fours<O>(more, a.p_count));
+                       (FORM == kWeightGrad && a.partial ? sixteens<float>(a.partial, a.p_count) : sixteens<O>(a.out[0], a.out_ld) && sixteens<O>(a.out[1], a.out_ld)) &&
+                       (!more || sixteens<O>(more, a.p_count));
 #define X(ACT) do { if (whole) finish<T, O, FORM, TWO, GRAD, S, ACT, true>(a, p0, q0, split, acc); else finish<T, O, FORM, TWO, GRAD, S, ACT, false>(a, p0, q0, split, acc); } while (0)
     if constexpr (FORM != kForward) {
         X(TGT_ACT_NONE);
