@@ -502,29 +502,33 @@ int tgt_nll_loss_bwd(const int64_t* d_target, const void* d_dloss, const float* 
 #define TGT_ACT_SILU 3
 /* h = act(x Wg^T + bg) * (x Wu^T + bu) */
 int tgt_gated_linear_fwd(const void* d_x, const void* d_Wg, const void* d_Wu, const void* d_bg, const void* d_bu, int64_t N,
-                         int in_features, int out_features, int dtype, int act, void* d_h, void* stream);
+                         int in_features, int out_features, int dtype, int act, void* d_h, void* d_kept, void* stream);
+/* Bytes of what a forward had better keep for its backward (both products, [N, 2 out_features] of `dtype`, 16-byte aligned) as
+ * d_kept; 0: nothing, the backward forms them again.  d_kept = NULL is always possible in a forward, and then in its backward. */
+int64_t tgt_gated_linear_kept_bytes(int64_t N, int in_features, int out_features, int dtype, int act);
 /* The same on operands in 8 bits (OCP e4m3): a value is its code times the scale of its row of x or of a weight.
  * in_features: a multiple of 16, d_x and the weights on 16-byte boundaries or not.  Biases and h are of `dtype`. */
 int tgt_gated_linear_8bit_fwd(const void* d_x, const float* d_x_scales, const void* d_Wg, const float* d_Wg_scales,
                               const void* d_Wu, const float* d_Wu_scales, const void* d_bg, const void* d_bu, int64_t N,
                               int in_features, int out_features, int dtype, int act, void* d_h, void* stream);
 /* Backward: d_dx [N, in_features] or NULL; d_dW: HOST array of the two weights' gradients, or NULL; d_db: HOST array of the
- * two biases' gradients (entries may be NULL), or NULL.  x, the weights and the biases are the forward's: what the
- * activation was taken of is formed again.  The sums over nodes are added in a fixed order (same inputs, same bits).
+ * two biases' gradients (entries may be NULL), or NULL.  x, the weights, the biases and d_kept are the forward's; without
+ * d_kept what the activation was taken of is formed again.  The sums over nodes are added in a fixed order (same inputs, same bits).
  * d_workspace: as many bytes as asked for, 16-byte aligned, contents need no initialisation.  N = 0: gradients of zero. */
 int64_t tgt_gated_linear_bwd_workspace_bytes(int64_t N, int in_features, int out_features, int dtype);
 int tgt_gated_linear_bwd(const void* d_x, const void* d_Wg, const void* d_Wu, const void* d_bg, const void* d_bu,
-                         const void* d_dh, int64_t N, int in_features, int out_features, int dtype, int act, void* d_dx,
-                         void* const* d_dW, void* const* d_db, void* d_workspace, int64_t workspace_bytes, void* stream);
-/* y = act(x W^T + b) + residual; residual [N, out_features] or NULL (its gradient is dy itself) */
+                         const void* d_dh, int64_t N, int in_features, int out_features, int dtype, int act, const void* d_kept,
+                         void* d_dx, void* const* d_dW, void* const* d_db, void* d_workspace, int64_t workspace_bytes, void* stream);
+/* y = act(x W^T + b) + residual; residual [N, out_features] or NULL (its gradient is dy itself); d_kept as above, [N, out_features] */
 int tgt_linear_epilogue_fwd(const void* d_x, const void* d_W, const void* d_b, const void* d_residual, int64_t N, int in_features,
-                            int out_features, int dtype, int act, void* d_y, void* stream);
+                            int out_features, int dtype, int act, void* d_y, void* d_kept, void* stream);
+int64_t tgt_linear_epilogue_kept_bytes(int64_t N, int in_features, int out_features, int dtype, int act);
 int tgt_linear_epilogue_8bit_fwd(const void* d_x, const float* d_x_scales, const void* d_W, const float* d_W_scales,
                                  const void* d_b, const void* d_residual, int64_t N, int in_features, int out_features, int dtype,
                                  int act, void* d_y, void* stream);
 int64_t tgt_linear_epilogue_bwd_workspace_bytes(int64_t N, int in_features, int out_features, int dtype, int act);
 int tgt_linear_epilogue_bwd(const void* d_x, const void* d_W, const void* d_b, const void* d_dy, int64_t N, int in_features,
-                            int out_features, int dtype, int act, void* d_dx, void* d_dW, void* d_db, void* d_workspace,
+                            int out_features, int dtype, int act, const void* d_kept, void* d_dx, void* d_dW, void* d_db, void* d_workspace,
                             int64_t workspace_bytes, void* stream);
 /* s = x (+ r), rounded to `dtype`; y = s / sqrt(mean(s^2) + eps) * weight.  d_sum: [N, C], NULL without a residual (s is x
  * then); d_rstd: float32 [N] for the backward, may be NULL.  C <= 16384. */

@@ -4,6 +4,8 @@ Every bound is a sum of what the arithmetic may lose, element by element:
   * a float32 sum of n terms: n 2^-23 of the sum of their magnitudes (the matrix instructions may cut instead of rounding; float32 operands in three
     parts leave out less than 2^-23 of a product: two more terms' worth);
   * a rounding to the tensors' type: eps / 2 of the value;
+  * where a forward keeps g and u for its backward (`kept`: float32 from 128 features on, bfloat16 from 512, where the kernels for small widths do not
+    take the call): their rounding to the tensors' type, in the gradients;
   * a function value: 2^-20 of the largest magnitude that goes into it (erff and expf are good to a few units of 2^-24), bfloat16 results 2^-14
     (v_exp_f32 of a product rounded to 24 bits);
   * operands in 8 bits: the matrix instruction adds eight neighbouring products at a time, aligned to the largest of them and cut 13 binary places below it
@@ -114,7 +116,14 @@ def gated_case(N, K, F, dt, act, bias, seed=0):
     return x, wg, wu, bg, bu, rand(g, N, F, dt=dt)
 
 
-def check_gated(x, wg, wu, bg, bu, dh, act, outs):
+class Rounded:
+    """A value with its error bound as it is read back from the tensors' type"""
+
+    def __init__(self, m, dt):
+        self.v, self.e = m.v, stored(m.v, m.e, dt)
+
+
+def check_gated(x, wg, wu, bg, bu, dh, act, outs, kept=False):
     dt = x.dtype
     X, WG, WU, BG, BU, DH = d(x), d(wg), d(wu), d(bg), d(bu), d(dh)
     g, u = Mapped(X, WG, BG), Mapped(X, WU, BU)
@@ -125,6 +134,9 @@ def check_gated(x, wg, wu, bg, bu, dh, act, outs):
     near(outs["h"], h, stored(h, eh, dt), "h")
     if dh is None:
         return
+    if kept:
+        g, u = Rounded(g, dt), Rounded(u, dt)
+        ea = 1.13 * g.e + fine(dt) * (g.v.abs() + g.e)
     s = slope64(act, g.v)
     es = curve(act, g.v, g.e) + fine(dt) * (1 + g.v.abs())
     dg, du = DH * u.v * s, DH * a
@@ -157,6 +169,52 @@ def run_gated(x, wg, wu, bg, bu, dh, act):
 def test_gated_linear(cuda, shape, dt, act, bias):
     case = gated_case(*shape, dt, act, bias)
     check_gated(*case, act, run_gated(*case, act))
+
+
+# Beyond the kernels for small widths: tiles of 128, what the forward keeps; whole rows, odd contractions, odd results
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("shape", [(300, 600, 900), (100, 1031, 520), (131, 640, 901), (65, 1040, 1024)])
+def test_wider_ones(cuda, shape, dt):
+    L, (N, K, F) = _lib.lib(), shape
+    code = _lib.DTYPE_F32 if dt == F32 else _lib.DTYPE_BF16
+    size = torch.finfo(dt).bits // 8
+    assert L.tgt_gated_linear_kept_bytes(N, K, F, code, 3) == N * 2 * F * size
+    case = gated_case(*shape, dt, "silu", True)
+    check_gated(*case, "silu", run_gated(*case, "silu"), kept=True)
+    kept = L.tgt_linear_epilogue_kept_bytes(N, K, F, code, 1)
+    assert kept in (0, N * F * size) and L.tgt_linear_epilogue_kept_bytes(N, K, F, code, 0) == 0
+    case = linear_case(*shape, dt, True, True)
+    check_linear(*case, "gelu", run_linear(*case, "gelu"), kept=kept > 0)
+    check_linear(*case, None, run_linear(*case, None))
+    with torch.no_grad():
+        x, w, b, r, _ = case
+        check_linear(x, w, b, r, None, "relu", {"y": T.linear_act(x, w, b, "relu", r)})
+
+
+def test_kept_or_formed_again(cuda):
+    """The C entry points take both ways at any size: kept values are the products rounded to the type, and the gradients of either way agree with the formula."""
+    L = _lib.lib()
+    st = torch.cuda.current_stream().cuda_stream
+    for dt, code in ((F32, 0), (BF16, 1)):
+        for N, K, F in ((40, 64, 48), (200, 72, 96), (200, 72, 97), (130, 520, 1032)):
+            x, wg, wu, bg, bu, dh = gated_case(N, K, F, dt, "silu", True)
+            P = [t.data_ptr() for t in (x, wg, wu, bg, bu)]
+            for keep in (False, True):
+                kept, h = torch.empty(N, 2 * F, device="cuda", dtype=dt), torch.empty(N, F, device="cuda", dtype=dt)
+                kp = kept.data_ptr() if keep else None
+                assert L.tgt_gated_linear_fwd(*P, N, K, F, code, 3, h.data_ptr(), kp, st) == 0
+                nbytes = L.tgt_gated_linear_bwd_workspace_bytes(N, K, F, code)
+                ws = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+                outs = {"h": h, "x": torch.empty_like(x), "wg": torch.empty_like(wg), "wu": torch.empty_like(wu), "bg": torch.empty_like(bg), "bu": torch.empty_like(bu)}
+                import ctypes
+                dW = (ctypes.c_void_p * 2)(outs["wg"].data_ptr(), outs["wu"].data_ptr())
+                db = (ctypes.c_void_p * 2)(outs["bg"].data_ptr(), outs["bu"].data_ptr())
+                assert L.tgt_gated_linear_bwd(*P, dh.data_ptr(), N, K, F, code, 3, kp, outs["x"].data_ptr(), dW, db, ws.data_ptr(), nbytes, st) == 0
+                check_gated(x, wg, wu, bg, bu, dh, "silu", outs, kept=keep)
+                if keep:
+                    for at, w, b in ((0, wg, bg), (F, wu, bu)):
+                        m = Mapped(d(x), d(w), d(b))
+                        near(kept[:, at:at + F], m.v, stored(m.v, m.e, dt), "kept")
 
 
 @pytest.mark.parametrize("dt", [F32, BF16])
@@ -240,7 +298,7 @@ def linear_case(N, K, M, dt, bias, residual):
             rand(g, N, M, dt=dt) if residual else None, rand(g, N, M, dt=dt))
 
 
-def check_linear(x, w, b, r, dy, act, outs, eight=False):
+def check_linear(x, w, b, r, dy, act, outs, eight=False, kept=False):
     dt = outs["y"].dtype
     X, W, B, R, DY = d(x), d(w), d(b), d(r), d(dy)
     u = Mapped(X, W, B, eight=eight)
@@ -254,6 +312,8 @@ def check_linear(x, w, b, r, dy, act, outs, eight=False):
     if act is None:
         du, edu = DY, torch.zeros_like(DY)
     else:
+        if kept:
+            u = Rounded(u, dt)
         du = DY * slope64(act, u.v)
         edu = stored(du, DY.abs() * (curve(act, u.v, u.e) + fine(dt) * (1 + u.v.abs())) + 2.0 ** -22 * du.abs(), dt)
     dx, dw = Mapped(du, W.T, ea=edu), Mapped(du.T, X.T, ea=edu.T)
@@ -714,7 +774,12 @@ def test_large_products_in_bf16(cuda, shape):
     check_linear(x[rows], wg, bg, dh[rows], None, "gelu", {"y": y["y"][rows]})
     check_linear(x[rows], wg, bg, dh[rows], None, None, {"y": yn["y"][rows]})
     WG, WU, BG, BU = d(wg), d(wu), d(bg), d(bu)
-    p, q = Mapped(X, WG, BG), Mapped(X, WU, BU)
+
+    def products(X, f=slice(None)):
+        p, q = Mapped(X, WG[f], BG[f]), Mapped(X, WU[f], BU[f])
+        return (Rounded(p, BF16), Rounded(q, BF16)) if K >= 512 else (p, q)
+
+    p, q = products(X)
     s, a = slope64("silu", p.v), act64("silu", p.v)
     dg, du = DH * q.v * s, DH * a
     edg = stored(dg, DH.abs() * (q.v.abs() * (0.8 * p.e + fine(BF16) * (1 + p.v.abs())) + (s.abs() + 0.8 * p.e) * q.e) + 2.0 ** -22 * dg.abs(), BF16)
@@ -726,7 +791,7 @@ def test_large_products_in_bf16(cuda, shape):
     # weight gradients: sampled rows f, the last among them
     fs = torch.cat([torch.tensor([0, F - 1, F - 2, (F - 1) // 256 * 256]), torch.randint(F, (12,), generator=g)])
     X, DH = d(x), d(dh[:, fs])
-    p, q = Mapped(X, WG[fs], BG[fs]), Mapped(X, WU[fs], BU[fs])
+    p, q = products(X, fs)
     s, a = slope64("silu", p.v), act64("silu", p.v)
     dg, du = DH * q.v * s, DH * a
     edg = stored(dg, DH.abs() * (q.v.abs() * (0.8 * p.e + fine(BF16) * (1 + p.v.abs())) + (s.abs() + 0.8 * p.e) * q.e) + 2.0 ** -22 * dg.abs(), BF16)

@@ -13,27 +13,27 @@ BAD, UNSUPPORTED, OK, WORKSPACE = _lib.ERR_INVALID_ARG, _lib.ERR_UNSUPPORTED, _l
 def test_entry_points_refuse_bad_arguments():
     L = _lib.lib()
     p = ctypes.c_void_p(4096)      # (never read: every call below ends before a launch)
-    assert L.tgt_gated_linear_fwd(p, p, p, None, None, -1, 8, 8, 0, 3, p, None) == BAD
-    assert L.tgt_gated_linear_fwd(p, p, p, None, None, 4, 0, 8, 0, 3, p, None) == BAD
-    assert L.tgt_gated_linear_fwd(p, p, p, None, None, 4, 8, 8, 2, 3, p, None) == BAD          # dtype
-    assert L.tgt_gated_linear_fwd(p, p, p, None, None, 4, 8, 8, 0, 4, p, None) == BAD          # activation
-    assert L.tgt_gated_linear_fwd(None, p, p, None, None, 4, 8, 8, 0, 3, p, None) == BAD
-    assert L.tgt_gated_linear_fwd(p, p, None, None, None, 4, 8, 8, 0, 3, p, None) == BAD
-    assert L.tgt_gated_linear_fwd(p, p, p, None, None, 4, 8, 8, 0, 3, None, None) == BAD
-    assert L.tgt_gated_linear_fwd(p, p, p, None, None, 1 << 31, 8, 8, 0, 3, p, None) == UNSUPPORTED
-    assert L.tgt_gated_linear_fwd(None, None, None, None, None, 0, 8, 8, 0, 3, None, None) == OK          # nothing to do
-    assert L.tgt_linear_epilogue_fwd(p, None, None, None, 4, 8, 8, 0, 0, p, None) == BAD
+    assert L.tgt_gated_linear_fwd(p, p, p, None, None, -1, 8, 8, 0, 3, p, None, None) == BAD
+    assert L.tgt_gated_linear_fwd(p, p, p, None, None, 4, 0, 8, 0, 3, p, None, None) == BAD
+    assert L.tgt_gated_linear_fwd(p, p, p, None, None, 4, 8, 8, 2, 3, p, None, None) == BAD          # dtype
+    assert L.tgt_gated_linear_fwd(p, p, p, None, None, 4, 8, 8, 0, 4, p, None, None) == BAD          # activation
+    assert L.tgt_gated_linear_fwd(None, p, p, None, None, 4, 8, 8, 0, 3, p, None, None) == BAD
+    assert L.tgt_gated_linear_fwd(p, p, None, None, None, 4, 8, 8, 0, 3, p, None, None) == BAD
+    assert L.tgt_gated_linear_fwd(p, p, p, None, None, 4, 8, 8, 0, 3, None, None, None) == BAD
+    assert L.tgt_gated_linear_fwd(p, p, p, None, None, 1 << 31, 8, 8, 0, 3, p, None, None) == UNSUPPORTED
+    assert L.tgt_gated_linear_fwd(None, None, None, None, None, 0, 8, 8, 0, 3, None, None, None) == OK          # nothing to do
+    assert L.tgt_linear_epilogue_fwd(p, None, None, None, 4, 8, 8, 0, 0, p, None, None) == BAD
     assert L.tgt_linear_epilogue_8bit_fwd(p, p, p, p, None, None, 4, 24, 8, 0, 0, p, None) == UNSUPPORTED
     assert L.tgt_linear_epilogue_8bit_fwd(p, None, p, p, None, None, 4, 32, 8, 0, 0, p, None) == BAD
     assert L.tgt_gated_linear_8bit_fwd(p, p, p, p, p, None, None, None, 4, 32, 8, 0, 0, p, None) == BAD
     dW = (ctypes.c_void_p * 2)(4096, None)
-    assert L.tgt_gated_linear_bwd(p, p, p, None, None, p, 4, 8, 8, 0, 3, p, dW, None, p, 1 << 20, None) == BAD      # one weight's gradient
-    assert L.tgt_gated_linear_bwd(p, p, p, None, None, None, 4, 8, 8, 0, 3, p, None, None, p, 1 << 20, None) == BAD
-    assert L.tgt_gated_linear_bwd(p, p, p, None, None, p, 4, 8, 8, 0, 3, p, None, None, None, 0, None) == WORKSPACE
+    assert L.tgt_gated_linear_bwd(p, p, p, None, None, p, 4, 8, 8, 0, 3, None, p, dW, None, p, 1 << 20, None) == BAD      # one weight's gradient
+    assert L.tgt_gated_linear_bwd(p, p, p, None, None, None, 4, 8, 8, 0, 3, None, p, None, None, p, 1 << 20, None) == BAD
+    assert L.tgt_gated_linear_bwd(p, p, p, None, None, p, 4, 8, 8, 0, 3, None, p, None, None, None, 0, None) == WORKSPACE
     need = L.tgt_gated_linear_bwd_workspace_bytes(1000, 64, 128, 0)
     assert need >= 1000 * 256 * 4
-    assert L.tgt_gated_linear_bwd(p, p, p, None, None, p, 1000, 64, 128, 0, 3, p, None, None, p, need - 16, None) == WORKSPACE
-    assert L.tgt_gated_linear_bwd(p, p, p, None, None, p, 1000, 64, 128, 0, 3, p, None, None, ctypes.c_void_p(4100), need, None) == WORKSPACE
+    assert L.tgt_gated_linear_bwd(p, p, p, None, None, p, 1000, 64, 128, 0, 3, None, p, None, None, p, need - 16, None) == WORKSPACE
+    assert L.tgt_gated_linear_bwd(p, p, p, None, None, p, 1000, 64, 128, 0, 3, None, p, None, None, ctypes.c_void_p(4100), need, None) == WORKSPACE
     assert L.tgt_gated_linear_bwd_workspace_bytes(-1, 64, 128, 0) == -1 and L.tgt_gated_linear_bwd_workspace_bytes(5, 64, 128, 7) == -1
     assert L.tgt_linear_epilogue_bwd_workspace_bytes(5, 0, 128, 0, 0) == -1
     assert L.tgt_add_rms_norm_fwd(p, None, p, 4, 0, 1e-6, 0, None, p, None, None) == BAD

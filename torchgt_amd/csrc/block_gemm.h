@@ -57,6 +57,7 @@ struct Args {
     const void* bias[2];       // [p_count] or null
     const void* residual;      // [q_count, p_count] or null
     const void* dy;            // kForward with GRAD: the gradient of the result
+    void* kept;                // kForward: what the activation and the other factor are taken of, [q_count][p_count of each weight], or null
     const float* q_scale;      // 8-bit operands: one per row of Q and of each P
     const float* p_scale[2];
     void* out[2];              // kWeightGrad: out[1] has the rows from q_first on

@@ -6,10 +6,10 @@
 // No counterpart in the reference, whose feed-forward block has one projection and a GELU (models/graphormer_dist_node_level.py:27-39).
 //
 // Backward.  With g = x Wg^T + bg, u = x Wu^T + bu:  dg = dh u act'(g), du = dh act(g);  dx = dg Wg + du Wu;  dWg = dg^T x, dWu = du^T x; biases: column
-// sums.  g and u are not kept from the forward: a first kernel forms them again in float32 and writes dg and du side by side, [N, 2F] (rounded to
-// the tensors' type, since they are operands of the next two products; that costs as much as the rounding of any other activation).  Keeping
-// them would cost 4 F values of memory per node and their rounding would go into act'.  dx and dW are products of what it wrote.
-// dW over few output tiles is cut along the nodes, partial sums in float32 added in a fixed order.
+// sums.  Where the contraction is long the forward keeps g and u (rounded to the tensors' type, like every activation of such a layer; h is formed of the
+// float32 values); where it is short they are not kept: a first kernel forms them again in float32.  Either writes dg and du, rounded to the tensors' type since
+// they are operands of the next two products; dx and dW are products of what it wrote.  dW over few output tiles is cut along the nodes, partial
+// sums in float32 added in a fixed order.
 #include "activations.h"
 #include "block_gemm.h"
 #include "gated_tiles.h"
@@ -66,6 +66,7 @@ __device__ __forceinline__ void finish(const Args& a, int64_t p0, int64_t q0, un
     constexpr bool kPair = FORM == kForward && TWO, EXACT = sizeof(O) == 4, kReads = FORM == kForward && (GRAD || !TWO);
     constexpr int kBy = kPair ? 2 : 1, kOut = S::FP / kBy;      // pieces that one output piece takes
     constexpr bool kWide = WHOLE && sizeof(O) == 2 && kOut % 2 == 0;
+    constexpr bool kKeeps = FORM == kForward && !GRAD && sizeof(T) > 1;
     constexpr int kGroup = kWide ? 2 : 1;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = (lane >> 4) * 4, row = lane & 15;
@@ -124,7 +125,7 @@ __device__ __forceinline__ void finish(const Args& a, int64_t p0, int64_t q0, un
             if constexpr (kWide && kReads) {
                 if (more) exchange(in[i0][j].v, in[i0 + 1][j].v);
             }
-            float o[kGroup][4], o2[kGroup][4];
+            float o[kGroup][4], o2[kGroup][4], keep[kBy][kGroup][4];
 #pragma unroll
             for (int n = 0; n < kGroup; ++n) {
                 const int i = i0 + n;
@@ -138,6 +139,7 @@ __device__ __forceinline__ void finish(const Args& a, int64_t p0, int64_t q0, un
                             float t = acc[i * kBy + w][j][e];
                             if constexpr (sizeof(T) == 1) t *= qs * scale[n][w][e];
                             v[w][e] = t + bias[n][w][e];
+                            if constexpr (kKeeps) keep[w][n][e] = v[w][e];
                         }
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
@@ -180,6 +182,13 @@ __device__ __forceinline__ void finish(const Args& a, int64_t p0, int64_t q0, un
                 put(reinterpret_cast<O*>(a.out[1]) + (q - a.q_first) * a.out_ld + p, o);
             } else {
                 put(reinterpret_cast<O*>(a.out[0]) + q * a.out_ld + p, o);
+                if constexpr (kKeeps) {
+                    if (a.kept) {
+                        O* to = reinterpret_cast<O*>(a.kept) + q * (kBy * a.p_count) + p;
+#pragma unroll
+                        for (int w = 0; w < kBy; ++w) put(to + w * a.p_count, keep[w]);
+                    }
+                }
                 if constexpr (GRAD && kPair) put(reinterpret_cast<O*>(a.out[1]) + q * a.out_ld + p, o2);
             }
         }
@@ -191,7 +200,7 @@ __device__ __forceinline__ void epilogue(const Args& a, int64_t p0, int64_t q0, 
     const void* more = GRAD ? a.dy : a.residual;
     const bool whole = p0 + kCols <= a.p_count && q0 + S::kRows <= a.q_count &&
                        (FORM == kWeightGrad && a.partial ? sixteens<float>(a.partial, a.p_count) : sixteens<O>(a.out[0], a.out_ld) && sixteens<O>(a.out[1], a.out_ld)) &&
-                       (!more || sixteens<O>(more, a.p_count));
+                       (!more || sixteens<O>(more, a.p_count)) && sixteens<O>(a.kept, a.p_count);
 #define X(ACT) do { if (whole) finish<T, O, FORM, TWO, GRAD, S, ACT, true>(a, p0, q0, split, acc); else finish<T, O, FORM, TWO, GRAD, S, ACT, false>(a, p0, q0, split, acc); } while (0)
     if constexpr (FORM != kForward) {
         X(TGT_ACT_NONE);
@@ -394,6 +403,80 @@ template <typename O> __global__ __launch_bounds__(256) void k_column_sums(const
     if (w == 0 && col < M) partial[blockIdx.y * M + col] = (part[0][c] + part[1][c]) + (part[2][c] + part[3][c]);
 }
 
+// dg = dh u act'(g), du = dh act(g) (one weight: du = dy act'(u)) from what the forward kept, [N, F] of each weight side by side, and the column sums of what is
+// written: workgroup (256 vectors of columns, share of the rows) -> partial[share][TWO ? 2 F : F] (null: not wanted).  Bound by memory: 16384 x
+// 4096 bf16, 671 MB.
+template <typename O, bool TWO, int ACT, int VE>
+__global__ __launch_bounds__(256) void k_kept_grad(const O* __restrict__ kept, const O* __restrict__ dy, int64_t N, int64_t F, int64_t rows_each, O* __restrict__ du,
+                                                   float* __restrict__ partial) {
+    constexpr int NW = TWO ? 2 : 1;
+    constexpr bool EXACT = sizeof(O) == 4;
+    struct alignas(VE * sizeof(O)) Some { O e[VE]; };
+    const int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * VE, r0 = blockIdx.y * rows_each, r1 = r0 + rows_each < N ? r0 + rows_each : N;
+    if (c >= F) return;
+    float sums[NW][VE];
+#pragma unroll
+    for (int w = 0; w < NW; ++w)
+#pragma unroll
+        for (int e = 0; e < VE; ++e) sums[w][e] = 0.f;
+    for (int64_t r = r0; r < r1; r += 2) {      // two rows in flight
+        Some in[2][NW + 1];
+        const int n = r + 1 < r1 ? 2 : 1;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int64_t row = i < n ? r + i : r;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) in[i][w] = *reinterpret_cast<const Some*>(kept + (row * NW + w) * F + c);
+            in[i][NW] = *reinterpret_cast<const Some*>(dy + row * F + c);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if (i >= n) break;
+            Some out[NW];
+#pragma unroll
+            for (int e = 0; e < VE; ++e) {
+                const float g = to_float(in[i][0].e[e]), d = to_float(in[i][NW].e[e]);
+                float o[NW];
+                if constexpr (TWO) {
+                    float f, s;
+                    act_and_slope<EXACT, ACT>(g, f, s);
+                    o[0] = d * to_float(in[i][1].e[e]) * s;
+                    o[NW - 1] = d * f;
+                } else o[0] = slope_of<EXACT, ACT>(g, d);
+#pragma unroll
+                for (int w = 0; w < NW; ++w) {
+                    sums[w][e] += o[w];
+                    from_float(out[w].e[e], o[w]);
+                }
+            }
+#pragma unroll
+            for (int w = 0; w < NW; ++w) *reinterpret_cast<Some*>(du + ((r + i) * NW + w) * F + c) = out[w];
+        }
+    }
+    if (!partial) return;
+#pragma unroll
+    for (int w = 0; w < NW; ++w)
+#pragma unroll
+        for (int e = 0; e < VE; ++e) partial[((int64_t)blockIdx.y * NW + w) * F + c + e] = sums[w][e];
+}
+template <typename O, bool TWO, int VE> void launch_kept_grad_as(const void* kept, const void* dy, int64_t N, int64_t F, int64_t rows_each, int shares, int act, void* du, float* partial, hipStream_t st) {
+    const dim3 grid((unsigned)((F + 256 * VE - 1) / (256 * VE)), (unsigned)shares);
+#define X(ACT) hipLaunchKernelGGL((k_kept_grad<O, TWO, ACT, VE>), grid, dim3(256), 0, st, (const O*)kept, (const O*)dy, N, F, rows_each, (O*)du, partial)
+    switch (act) {
+        case TGT_ACT_SILU: X(TGT_ACT_SILU); break;
+        case TGT_ACT_GELU: X(TGT_ACT_GELU); break;
+        case TGT_ACT_RELU: X(TGT_ACT_RELU); break;
+        default: X(TGT_ACT_NONE); break;
+    }
+#undef X
+}
+template <typename O> void launch_kept_grad(const void* kept, const void* dy, int n, int64_t N, int64_t F, int64_t rows_each, int shares, int act, void* du, float* partial, hipStream_t st) {
+    constexpr int VE = 16 / (int)sizeof(O);
+    const bool whole = F % VE == 0 && (((uintptr_t)kept | (uintptr_t)dy | (uintptr_t)du) & 15) == 0;
+    if (n == 2) return whole ? launch_kept_grad_as<O, true, VE>(kept, dy, N, F, rows_each, shares, act, du, partial, st) : launch_kept_grad_as<O, true, 1>(kept, dy, N, F, rows_each, shares, act, du, partial, st);
+    return whole ? launch_kept_grad_as<O, false, VE>(kept, dy, N, F, rows_each, shares, act, du, partial, st) : launch_kept_grad_as<O, false, 1>(kept, dy, N, F, rows_each, shares, act, du, partial, st);
+}
+
 // Rows F .. Fp - 1 of a weight are zeros
 template <typename O> __global__ __launch_bounds__(256) void k_pad_rows(const O* __restrict__ w, int64_t n, int64_t all, O* __restrict__ out) {
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) out[i] = i < n ? w[i] : O{};
@@ -585,6 +668,7 @@ Args forward_args(const Call& c) {
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+bool needs_du(int n, int act) { return n == 2 || act != TGT_ACT_NONE; }      // (else dy is the operand itself)
 int in16(int dtype) { return dtype == TGT_DTYPE_F32 ? 4 : 8; }      // elements in 16 bytes
 // Whether the kernels for small widths (gated_tiles.hip, linear_tiles.hip) are the faster ones: weights of up to a million values and, forward + backward in us,
 // those kernels / the tiles of 128 and 256:   float32   300 x 128 x 128 25 / 59    2000 x 1024 x 1024 166 / 275   64000 x 256 x 256 206 / 236
@@ -604,11 +688,16 @@ NarrowArgs narrow_args(const Call& c, const void* more) {
     return a;
 }
 
-int forward(const Call& c, const void* residual, void* out, hipStream_t st) {
+// What a forward that will have a backward is asked to keep: the products themselves, where forming them again takes longer than writing and reading them.
+// us of the gradients formed again / kept and read (with what the forward takes longer), bf16 16384 rows of K to 4096: see the end of this file's
+// comments on k_kept_grad; about 4 K / 1.2e15 + 2e-12 s a value against 3e-12.
+bool keeps(const Call& c) { return needs_du(c.n, c.act) && c.N > 64 && !narrow(c) && c.K >= (c.dtype == TGT_DTYPE_F32 ? 128 : 512); }
+
+int forward(const Call& c, const void* residual, void* out, void* kept, hipStream_t st) {
     int rc = check_call(c);
     if (rc != TGT_OK || c.N == 0) return rc;
     if (!out) { set_error("%s: null pointer", c.who); return TGT_ERR_INVALID_ARG; }
-    if (c.N > 64 && narrow(c)) {
+    if (c.N > 64 && narrow(c) && !kept) {
         NarrowArgs a = narrow_args(c, residual);
         a.out[0] = out;
         KernelTimer t(KS_LINEAR_FWD, st);
@@ -617,6 +706,7 @@ int forward(const Call& c, const void* residual, void* out, hipStream_t st) {
     Args a = forward_args(c);
     a.residual = residual;
     a.out[0] = out;
+    a.kept = kept;
     KernelTimer t(KS_LINEAR_FWD, st);
     return c.dtype == TGT_DTYPE_F32 ? product_forward<float, float>(a, false, st) : product_forward<b16, b16>(a, false, st);
 }
@@ -655,7 +745,7 @@ Plan plan_of(int n, int64_t N, int K, int F, int dtype, int act) {
     const int64_t want = std::max<int64_t>(1, std::min<int64_t>((512 + tiles - 1) / tiles, (N + 8 * step - 1) / (8 * step)));
     p.K_each = ((N + want - 1) / std::max<int64_t>(1, want) + step - 1) / step * step;
     p.splits = N > 0 ? (int)((N + p.K_each - 1) / p.K_each) : 1;
-    p.shares = (int)std::max<int64_t>(1, std::min<int64_t>(256, (N + 127) / 128));
+    p.shares = (int)std::max<int64_t>(1, std::min<int64_t>(512, (N + 31) / 32));
     p.rows_each = (N + p.shares - 1) / p.shares;
     p.bytes = p.du_bytes + (p.splits > 1 ? up16((int64_t)p.splits * cols * K * 4) : 0) + up16((int64_t)p.shares * cols * 4);
     return p;
@@ -666,7 +756,6 @@ int64_t workspace_bytes_of(int n, int64_t N, int K, int F, int dtype, int act);
 // The backward where the widths are small: one kernel for dg and du, rows of 16 bytes, then the linears' own backward of two weights of one shape (which reads them
 // once for dx and once for all weight and bias gradients)
 int padded_width(int F, int dtype) { return (F + in16(dtype) - 1) / in16(dtype) * in16(dtype); }
-bool needs_du(int n, int act) { return n == 2 || act != TGT_ACT_NONE; }
 int64_t narrow_bytes(int n, int64_t N, int K, int F, int dtype, int act) {
     const int64_t Fp = padded_width(F, dtype), size = dtype == TGT_DTYPE_F32 ? 4 : 2;
     return (needs_du(n, act) ? n * up16(N * Fp * size) : 0) + (Fp != F ? up16(Fp * K * size) : 0) + up16(tgt_linear_bwd_workspace_bytes(n, K, (int)Fp));
@@ -715,7 +804,7 @@ bool narrow_backward(const Call& c, const void* dy) {
     return narrow(c) && (padded_width(c.F, c.dtype) == c.F || (c.n == 1 && c.act != TGT_ACT_NONE)) && (needs_du(c.n, c.act) || aligned16(dy));
 }
 
-int backward(const Call& c, const void* dy, void* dx, void* const* dW, void* const* db, void* workspace, int64_t workspace_bytes, hipStream_t st) {
+int backward(const Call& c, const void* kept, const void* dy, void* dx, void* const* dW, void* const* db, void* workspace, int64_t workspace_bytes, hipStream_t st) {
     int rc = check_call(c);
     if (rc != TGT_OK) return rc;
     const bool f32 = c.dtype == TGT_DTYPE_F32;
@@ -739,9 +828,16 @@ int backward(const Call& c, const void* dy, void* dx, void* const* dW, void* con
         return TGT_ERR_WORKSPACE;
     }
     char* ws = (char*)workspace;
-    if (narrow_backward(c, dy)) return backward_narrow(c, dy, dx, dW, db, ws, st);
+    if (!kept && narrow_backward(c, dy)) return backward_narrow(c, dy, dx, dW, db, ws, st);
     const void* du = dy;
-    if (p.du_bytes) {
+    float* sums = (float*)(ws + p.bytes - up16((int64_t)p.shares * cols * 4));
+    if (p.du_bytes && kept) {
+        KernelTimer t(KS_GELU, st);
+        if (f32) launch_kept_grad<float>(kept, dy, c.n, c.N, c.F, p.rows_each, p.shares, c.act, ws, want_b ? sums : nullptr, st);
+        else launch_kept_grad<b16>(kept, dy, c.n, c.N, c.F, p.rows_each, p.shares, c.act, ws, want_b ? sums : nullptr, st);
+        TGT_HIP_CHECK(hipGetLastError());
+        du = ws;
+    } else if (p.du_bytes) {
         Args a = forward_args(c);
         a.dy = dy;
         a.out[0] = ws;
@@ -796,13 +892,14 @@ int backward(const Call& c, const void* dy, void* dx, void* const* dW, void* con
         }
     }
     if (want_b) {
-        float* partial = (float*)(ws + p.bytes - up16((int64_t)p.shares * cols * 4));
-        const dim3 grid((unsigned)((cols + 63) / 64), (unsigned)p.shares);
-        if (f32) hipLaunchKernelGGL((k_column_sums<float>), grid, dim3(256), 0, st, (const float*)du, c.N, cols, p.rows_each, partial);
-        else hipLaunchKernelGGL((k_column_sums<b16>), grid, dim3(256), 0, st, (const b16*)du, c.N, cols, p.rows_each, partial);
-        TGT_HIP_CHECK(hipGetLastError());
+        if (!(p.du_bytes && kept)) {
+            const dim3 grid((unsigned)((cols + 63) / 64), (unsigned)p.shares);
+            if (f32) hipLaunchKernelGGL((k_column_sums<float>), grid, dim3(256), 0, st, (const float*)du, c.N, cols, p.rows_each, sums);
+            else hipLaunchKernelGGL((k_column_sums<b16>), grid, dim3(256), 0, st, (const b16*)du, c.N, cols, p.rows_each, sums);
+            TGT_HIP_CHECK(hipGetLastError());
+        }
         tgt_reduce_desc r{};
-        r.partial = partial; r.workers = p.shares; r.n = (int)cols; r.n_out = c.n;
+        r.partial = sums; r.workers = p.shares; r.n = (int)cols; r.n_out = c.n;
         r.out[0] = db[0]; r.begin[0] = 0;
         if (c.n == 2) { r.out[1] = db[1]; r.begin[1] = c.F; }
         return reduce_partials(&r, 1, c.dtype, st);
@@ -810,6 +907,11 @@ int backward(const Call& c, const void* dy, void* dx, void* const* dW, void* con
     return TGT_OK;
 }
 
+int64_t kept_bytes_of(int n, int64_t N, int K, int F, int dtype, int act) {
+    if (N < 0 || K < 1 || F < 1 || (dtype != TGT_DTYPE_F32 && dtype != TGT_DTYPE_BF16)) return -1;
+    const Call c{"", nullptr, {nullptr, nullptr}, {nullptr, nullptr}, n, N, K, F, dtype, act};
+    return keeps(c) ? N * n * F * (dtype == TGT_DTYPE_F32 ? 4 : 2) : 0;
+}
 int64_t workspace_bytes_of(int n, int64_t N, int K, int F, int dtype, int act) {
     if (N < 0 || K < 1 || F < 1 || (dtype != TGT_DTYPE_F32 && dtype != TGT_DTYPE_BF16)) return -1;
     if (N == 0) return 0;
@@ -827,9 +929,12 @@ int64_t workspace_bytes_of(int n, int64_t N, int K, int F, int dtype, int act) {
 extern "C" {
 
 int tgt_gated_linear_fwd(const void* d_x, const void* d_Wg, const void* d_Wu, const void* d_bg, const void* d_bu, int64_t N, int in_features, int out_features,
-                         int dtype, int act, void* d_h, void* stream) {
+                         int dtype, int act, void* d_h, void* d_kept, void* stream) {
     const tgt::Call c{"tgt_gated_linear_fwd", d_x, {d_Wg, d_Wu}, {d_bg, d_bu}, 2, N, in_features, out_features, dtype, act};
-    return tgt::forward(c, nullptr, d_h, (hipStream_t)stream);
+    return tgt::forward(c, nullptr, d_h, d_kept, (hipStream_t)stream);
+}
+int64_t tgt_gated_linear_kept_bytes(int64_t N, int in_features, int out_features, int dtype, int act) {
+    return tgt::kept_bytes_of(2, N, in_features, out_features, dtype, act);
 }
 int tgt_gated_linear_8bit_fwd(const void* d_x, const float* d_x_scales, const void* d_Wg, const float* d_Wg_scales, const void* d_Wu, const float* d_Wu_scales,
                               const void* d_bg, const void* d_bu, int64_t N, int in_features, int out_features, int dtype, int act, void* d_h, void* stream) {
@@ -840,16 +945,19 @@ int64_t tgt_gated_linear_bwd_workspace_bytes(int64_t N, int in_features, int out
     return tgt::workspace_bytes_of(2, N, in_features, out_features, dtype, TGT_ACT_SILU);
 }
 int tgt_gated_linear_bwd(const void* d_x, const void* d_Wg, const void* d_Wu, const void* d_bg, const void* d_bu, const void* d_dh, int64_t N, int in_features,
-                         int out_features, int dtype, int act, void* d_dx, void* const* d_dW, void* const* d_db, void* d_workspace, int64_t workspace_bytes,
-                         void* stream) {
+                         int out_features, int dtype, int act, const void* d_kept, void* d_dx, void* const* d_dW, void* const* d_db, void* d_workspace,
+                         int64_t workspace_bytes, void* stream) {
     const tgt::Call c{"tgt_gated_linear_bwd", d_x, {d_Wg, d_Wu}, {d_bg, d_bu}, 2, N, in_features, out_features, dtype, act};
-    return tgt::backward(c, d_dh, d_dx, d_dW, d_db, d_workspace, workspace_bytes, (hipStream_t)stream);
+    return tgt::backward(c, d_kept, d_dh, d_dx, d_dW, d_db, d_workspace, workspace_bytes, (hipStream_t)stream);
 }
 
 int tgt_linear_epilogue_fwd(const void* d_x, const void* d_W, const void* d_b, const void* d_residual, int64_t N, int in_features, int out_features, int dtype,
-                            int act, void* d_y, void* stream) {
+                            int act, void* d_y, void* d_kept, void* stream) {
     const tgt::Call c{"tgt_linear_epilogue_fwd", d_x, {d_W, nullptr}, {d_b, nullptr}, 1, N, in_features, out_features, dtype, act};
-    return tgt::forward(c, d_residual, d_y, (hipStream_t)stream);
+    return tgt::forward(c, d_residual, d_y, d_kept, (hipStream_t)stream);
+}
+int64_t tgt_linear_epilogue_kept_bytes(int64_t N, int in_features, int out_features, int dtype, int act) {
+    return tgt::kept_bytes_of(1, N, in_features, out_features, dtype, act);
 }
 int tgt_linear_epilogue_8bit_fwd(const void* d_x, const float* d_x_scales, const void* d_W, const float* d_W_scales, const void* d_b, const void* d_residual,
                                  int64_t N, int in_features, int out_features, int dtype, int act, void* d_y, void* stream) {
@@ -860,10 +968,10 @@ int64_t tgt_linear_epilogue_bwd_workspace_bytes(int64_t N, int in_features, int 
     return tgt::workspace_bytes_of(1, N, in_features, out_features, dtype, act);
 }
 int tgt_linear_epilogue_bwd(const void* d_x, const void* d_W, const void* d_b, const void* d_dy, int64_t N, int in_features, int out_features, int dtype, int act,
-                            void* d_dx, void* d_dW, void* d_db, void* d_workspace, int64_t workspace_bytes, void* stream) {
+                            const void* d_kept, void* d_dx, void* d_dW, void* d_db, void* d_workspace, int64_t workspace_bytes, void* stream) {
     const tgt::Call c{"tgt_linear_epilogue_bwd", d_x, {d_W, nullptr}, {d_b, nullptr}, 1, N, in_features, out_features, dtype, act};
     void *dW[2] = {d_dW, nullptr}, *db[2] = {d_db, nullptr};
-    return tgt::backward(c, d_dy, d_dx, dW, db, d_workspace, workspace_bytes, (hipStream_t)stream);
+    return tgt::backward(c, d_kept, d_dy, d_dx, dW, db, d_workspace, workspace_bytes, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -160,11 +160,13 @@ void check_residual(const Optional& r, const Tensor& x, at::ScalarType type, int
     TORCH_CHECK(r->scalar_type() == type && r->sizes() == at::IntArrayRef(with_last(x, F)), op, ": residual must be ", type, " of the result's shape");
 }
 
-Tensor gated_forward(const Tensor& x, const Tensor& wg, const Tensor& wu, const Optional& bg, const Optional& bu, const RowsOf& rows, int64_t act) {
+// kept: null, or where to put what the forward keeps for a backward
+Tensor gated_forward(const Tensor& x, const Tensor& wg, const Tensor& wu, const Optional& bg, const Optional& bu, const RowsOf& rows, int64_t act, Tensor* kept) {
     const int64_t F = wg.size(0);
     Tensor h = at::empty(with_last(x, F), x.options());
+    if (kept && tgt_gated_linear_kept_bytes(rows.N, (int)rows.C, (int)F, dtype_code(x), (int)act) > 0) *kept = at::empty({rows.N, 2 * F}, x.options());
     check(tgt_gated_linear_fwd(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), ptr(bg), ptr(bu), rows.N, (int)rows.C, (int)F, dtype_code(x), (int)act, h.data_ptr(),
-                               stream_of(x)),
+                               kept && kept->defined() ? kept->data_ptr() : nullptr, stream_of(x)),
           "tgt_gated_linear_fwd");
     return h;
 }
@@ -174,8 +176,8 @@ struct GatedLinear : public torch::autograd::Function<GatedLinear> {
         c10::DeviceGuard guard(x.device());
         Tensor x2 = x.contiguous(), g2 = wg.contiguous(), u2 = wu.contiguous();
         Optional b1 = compact(bg), b2 = compact(bu);
-        Tensor h = gated_forward(x2, g2, u2, b1, b2, rows, act);
-        ctx->save_for_backward({x2, g2, u2, given(b1) ? *b1 : Tensor(), given(b2) ? *b2 : Tensor()});
+        Tensor kept, h = gated_forward(x2, g2, u2, b1, b2, rows, act, &kept);
+        ctx->save_for_backward({x2, g2, u2, given(b1) ? *b1 : Tensor(), given(b2) ? *b2 : Tensor(), kept});
         ctx->saved_data["act"] = act;
         ctx->saved_data["dx"] = x.requires_grad();
         ctx->saved_data["dw"] = wg.requires_grad() || wu.requires_grad();
@@ -185,7 +187,7 @@ struct GatedLinear : public torch::autograd::Function<GatedLinear> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         once("gated_linear");
         auto saved = ctx->get_saved_variables();
-        const Tensor &x = saved[0], &wg = saved[1], &wu = saved[2], &bg = saved[3], &bu = saved[4];
+        const Tensor &x = saved[0], &wg = saved[1], &wu = saved[2], &bg = saved[3], &bu = saved[4], &kept = saved[5];
         const int64_t F = wg.size(0), C = wg.size(1), N = x.numel() / C, act = ctx->saved_data["act"].toInt(), biases = ctx->saved_data["db"].toInt();
         c10::DeviceGuard guard(x.device());
         Tensor dh = grads[0].contiguous(), dx, dwg, dwu, dbg, dbu;
@@ -198,7 +200,7 @@ struct GatedLinear : public torch::autograd::Function<GatedLinear> {
         const int64_t nbytes = tgt_gated_linear_bwd_workspace_bytes(N, (int)C, (int)F, dtype_code(x));
         Tensor ws = at::empty({nbytes}, x.options().dtype(at::kByte));
         check(tgt_gated_linear_bwd(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), at_of(bg), at_of(bu), dh.data_ptr(), N, (int)C, (int)F, dtype_code(x), (int)act,
-                                   at_of(dx), dW, db, ws.data_ptr(), nbytes, stream_of(x)),
+                                   at_of(kept), at_of(dx), dW, db, ws.data_ptr(), nbytes, stream_of(x)),
               "tgt_gated_linear_bwd");
         return {dx, dwg, dwu, dbg, dbu, Tensor()};
     }
@@ -219,13 +221,15 @@ Tensor gated_linear(const Tensor& x, const Tensor& wg, const Tensor& wu, const O
     if (given(bu)) want.look(*bu);
     if (want.node()) return GatedLinear::apply(x, wg, wu, bg, bu, act);
     c10::DeviceGuard guard(x.device());
-    return gated_forward(x.contiguous(), wg.contiguous(), wu.contiguous(), compact(bg), compact(bu), rows, act);
+    return gated_forward(x.contiguous(), wg.contiguous(), wu.contiguous(), compact(bg), compact(bu), rows, act, nullptr);
 }
 
-Tensor linear_act_forward(const Tensor& x, const Tensor& w, const Optional& b, const Optional& r, const RowsOf& rows, int64_t act) {
+Tensor linear_act_forward(const Tensor& x, const Tensor& w, const Optional& b, const Optional& r, const RowsOf& rows, int64_t act, Tensor* kept) {
     const int64_t F = w.size(0);
     Tensor y = at::empty(with_last(x, F), x.options());
-    check(tgt_linear_epilogue_fwd(x.data_ptr(), w.data_ptr(), ptr(b), ptr(r), rows.N, (int)rows.C, (int)F, dtype_code(x), (int)act, y.data_ptr(), stream_of(x)),
+    if (kept && tgt_linear_epilogue_kept_bytes(rows.N, (int)rows.C, (int)F, dtype_code(x), (int)act) > 0) *kept = at::empty({rows.N, F}, x.options());
+    check(tgt_linear_epilogue_fwd(x.data_ptr(), w.data_ptr(), ptr(b), ptr(r), rows.N, (int)rows.C, (int)F, dtype_code(x), (int)act, y.data_ptr(),
+                                  kept && kept->defined() ? kept->data_ptr() : nullptr, stream_of(x)),
           "tgt_linear_epilogue_fwd");
     return y;
 }
@@ -235,8 +239,8 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
         c10::DeviceGuard guard(x.device());
         Tensor x2 = x.contiguous(), w2 = w.contiguous();
         Optional b2 = compact(b);
-        Tensor y = linear_act_forward(x2, w2, b2, compact(r), rows, act);
-        ctx->save_for_backward({x2, w2, given(b2) ? *b2 : Tensor()});
+        Tensor kept, y = linear_act_forward(x2, w2, b2, compact(r), rows, act, &kept);
+        ctx->save_for_backward({x2, w2, given(b2) ? *b2 : Tensor(), kept});
         ctx->saved_data["act"] = act;
         ctx->saved_data["dx"] = x.requires_grad();
         ctx->saved_data["dw"] = w.requires_grad();
@@ -247,7 +251,7 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         once("linear_act");
         auto saved = ctx->get_saved_variables();
-        const Tensor &x = saved[0], &w = saved[1], &b = saved[2];
+        const Tensor &x = saved[0], &w = saved[1], &b = saved[2], &kept = saved[3];
         const int64_t F = w.size(0), C = w.size(1), N = x.numel() / C, act = ctx->saved_data["act"].toInt();
         c10::DeviceGuard guard(x.device());
         Tensor dx, dw, db;
@@ -260,7 +264,7 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
             const int64_t nbytes = tgt_linear_epilogue_bwd_workspace_bytes(N, (int)C, (int)F, dtype_code(x), (int)act);
             Tensor ws = at::empty({nbytes}, x.options().dtype(at::kByte));
             auto at_of = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
-            check(tgt_linear_epilogue_bwd(x.data_ptr(), w.data_ptr(), at_of(b), dy.data_ptr(), N, (int)C, (int)F, dtype_code(x), (int)act, at_of(dx), at_of(dw),
+            check(tgt_linear_epilogue_bwd(x.data_ptr(), w.data_ptr(), at_of(b), dy.data_ptr(), N, (int)C, (int)F, dtype_code(x), (int)act, at_of(kept), at_of(dx), at_of(dw),
                                           at_of(db), ws.data_ptr(), nbytes, stream_of(x)),
                   "tgt_linear_epilogue_bwd");
         }
@@ -282,7 +286,7 @@ Tensor linear_act(const Tensor& x, const Tensor& w, const Optional& b, const Opt
     if (given(r)) want.look(*r);
     if (want.node()) return LinearAct::apply(x, w, b, r, act);
     c10::DeviceGuard guard(x.device());
-    return linear_act_forward(x.contiguous(), w.contiguous(), compact(b), compact(r), rows, act);
+    return linear_act_forward(x.contiguous(), w.contiguous(), compact(b), compact(r), rows, act, nullptr);
 }
 
 // ---- operands in 8 bits --------------------------------------------------------------------------------------------------------------------
