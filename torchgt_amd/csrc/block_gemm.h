@@ -43,6 +43,13 @@ template <> struct Kind<b16> { static constexpr int kPlanes = 1, kStep = 64, kPi
 template <> struct Kind<float> { static constexpr int kPlanes = 3, kStep = 32, kPiece = 8, kRowBytes = 64; };
 template <> struct Kind<e4m3> { static constexpr int kPlanes = 1, kStep = 128, kPiece = 16, kRowBytes = 128; };
 
+// The lane, as a value the compiler knows nothing of: what is made of it between two tiles is made there, and not kept in registers through the products
+__device__ __forceinline__ int fresh_lane() {
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    return lane;
+}
+
 enum Form { kForward, kInputGrad, kWeightGrad };
 
 struct Args {
@@ -446,7 +453,7 @@ template <typename T, bool KC, int HALVES> struct Feed {
 
     // PAIR: 16 rows of the first matrix, 16 of the second (KC).  Rows and columns behind the last are read from the last.
     template <bool PAIR> __device__ __forceinline__ void begin(const void* m0, const void* m1, int64_t ld, int64_t first, int64_t count, int64_t k0) {
-        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int lane = fresh_lane(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const T* m = reinterpret_cast<const T*>(PAIR && (wave & 2) ? m1 : m0);      // (pieces `wave` and `wave + 8`: 16 rows are two pieces)
         const char* start = reinterpret_cast<const char*>(m + (KC ? first * ld + k0 : k0 * ld + first));
         step = (KC ? Kind<T>::kStep : Kind<T>::kStep * ld) * (int64_t)sizeof(T);

@@ -68,7 +68,7 @@ __device__ __forceinline__ void finish(const Args& a, int64_t p0, int64_t q0, un
     constexpr bool kWide = WHOLE && sizeof(O) == 2 && kOut % 2 == 0;
     constexpr bool kKeeps = FORM == kForward && !GRAD && sizeof(T) > 1;
     constexpr int kGroup = kWide ? 2 : 1;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = fresh_lane(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = (lane >> 4) * 4, row = lane & 15;
     const int wide_col = ((lane >> 4) & 1) * 16 + (lane >> 5) * 8;      // of 32
     const O* more = reinterpret_cast<const O*>(GRAD ? a.dy : a.residual);
@@ -567,8 +567,9 @@ template <typename T, typename O> int product_forward(const Args& a, bool grad, 
 #undef X
     }
     if constexpr (sizeof(T) < 4) {
-        if (al && wide_enough(a, two ? 128 : 256, 1)) {
-#define X(TWO, GRAD) if (two == TWO && grad == GRAD) return launch_wide<T, O, kForward, TWO, GRAD, Wide<2>>(a, 1, st)
+        constexpr int PH = sizeof(T) == 1 ? 1 : 2;
+        if (al && wide_enough(a, (two ? 64 : 128) * PH, 1)) {
+#define X(TWO, GRAD) if (two == TWO && grad == GRAD) return launch_wide<T, O, kForward, TWO, GRAD, Wide<PH>>(a, 1, st)
             X(false, false); X(true, false);
             if constexpr (sizeof(T) > 1) { X(false, true); X(true, true); }
 #undef X
