@@ -497,12 +497,16 @@ int tgt_nll_loss_bwd(const int64_t* d_target, const void* d_dloss, const float* 
  *
  * act: TGT_ACT_NONE, TGT_ACT_GELU (exact erf form), TGT_ACT_RELU or TGT_ACT_SILU (u / (1 + exp(-u))).
  * d_x: [N, in_features]; weights [out_features, in_features] (nn.Linear.weight); biases [out_features] or NULL;
- * outputs [N, out_features]; all of `dtype` and at any address of that type; sums in float32.  N < 2^31. */
+ * outputs [N, out_features]; all of `dtype` and at any address of that type; sums in float32.  N < 2^31.
+ * d_workspace of a forward (sums of a contraction cut in pieces, where there are few rows): as many bytes as asked for, 16-byte
+ * aligned, contents need no initialisation; may be NULL where that is 0. */
 #define TGT_ACT_NONE 0
 #define TGT_ACT_SILU 3
 /* h = act(x Wg^T + bg) * (x Wu^T + bu) */
 int tgt_gated_linear_fwd(const void* d_x, const void* d_Wg, const void* d_Wu, const void* d_bg, const void* d_bu, int64_t N,
-                         int in_features, int out_features, int dtype, int act, void* d_h, void* d_kept, void* stream);
+                         int in_features, int out_features, int dtype, int act, void* d_h, void* d_kept, void* d_workspace,
+                         int64_t workspace_bytes, void* stream);
+int64_t tgt_gated_linear_fwd_workspace_bytes(int64_t N, int in_features, int out_features, int dtype);
 /* Bytes of what a forward had better keep for its backward (both products, [N, 2 out_features] of `dtype`, 16-byte aligned) as
  * d_kept; 0: nothing, the backward forms them again.  d_kept = NULL is always possible in a forward, and then in its backward. */
 int64_t tgt_gated_linear_kept_bytes(int64_t N, int in_features, int out_features, int dtype, int act);
@@ -510,7 +514,9 @@ int64_t tgt_gated_linear_kept_bytes(int64_t N, int in_features, int out_features
  * in_features: a multiple of 16, d_x and the weights on 16-byte boundaries or not.  Biases and h are of `dtype`. */
 int tgt_gated_linear_8bit_fwd(const void* d_x, const float* d_x_scales, const void* d_Wg, const float* d_Wg_scales,
                               const void* d_Wu, const float* d_Wu_scales, const void* d_bg, const void* d_bu, int64_t N,
-                              int in_features, int out_features, int dtype, int act, void* d_h, void* stream);
+                              int in_features, int out_features, int dtype, int act, void* d_h, void* d_workspace, int64_t workspace_bytes,
+                              void* stream);
+int64_t tgt_gated_linear_8bit_workspace_bytes(int64_t N, int in_features, int out_features);
 /* Backward: d_dx [N, in_features] or NULL; d_dW: HOST array of the two weights' gradients, or NULL; d_db: HOST array of the
  * two biases' gradients (entries may be NULL), or NULL.  x, the weights, the biases and d_kept are the forward's; without
  * d_kept what the activation was taken of is formed again.  The sums over nodes are added in a fixed order (same inputs, same bits).
@@ -521,11 +527,13 @@ int tgt_gated_linear_bwd(const void* d_x, const void* d_Wg, const void* d_Wu, co
                          void* d_dx, void* const* d_dW, void* const* d_db, void* d_workspace, int64_t workspace_bytes, void* stream);
 /* y = act(x W^T + b) + residual; residual [N, out_features] or NULL (its gradient is dy itself); d_kept as above, [N, out_features] */
 int tgt_linear_epilogue_fwd(const void* d_x, const void* d_W, const void* d_b, const void* d_residual, int64_t N, int in_features,
-                            int out_features, int dtype, int act, void* d_y, void* d_kept, void* stream);
+                            int out_features, int dtype, int act, void* d_y, void* d_kept, void* d_workspace, int64_t workspace_bytes, void* stream);
+int64_t tgt_linear_epilogue_fwd_workspace_bytes(int64_t N, int in_features, int out_features, int dtype);
 int64_t tgt_linear_epilogue_kept_bytes(int64_t N, int in_features, int out_features, int dtype, int act);
 int tgt_linear_epilogue_8bit_fwd(const void* d_x, const float* d_x_scales, const void* d_W, const float* d_W_scales,
                                  const void* d_b, const void* d_residual, int64_t N, int in_features, int out_features, int dtype,
-                                 int act, void* d_y, void* stream);
+                                 int act, void* d_y, void* d_workspace, int64_t workspace_bytes, void* stream);
+int64_t tgt_linear_epilogue_8bit_workspace_bytes(int64_t N, int in_features, int out_features);
 int64_t tgt_linear_epilogue_bwd_workspace_bytes(int64_t N, int in_features, int out_features, int dtype, int act);
 int tgt_linear_epilogue_bwd(const void* d_x, const void* d_W, const void* d_b, const void* d_dy, int64_t N, int in_features,
                             int out_features, int dtype, int act, const void* d_kept, void* d_dx, void* d_dW, void* d_db, void* d_workspace,

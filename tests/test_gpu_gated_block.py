@@ -191,6 +191,26 @@ def test_wider_ones(cuda, shape, dt):
         check_linear(x, w, b, r, None, "relu", {"y": T.linear_act(x, w, b, "relu", r)})
 
 
+# Few tiles and a long contraction, cut in pieces whose sums are joined: rows and columns that end inside a tile or a piece of one, contractions that end inside
+# a step and that change from one weight to the other inside and at the border of a piece, operands at odd addresses
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("shape", [(65, 1536, 712), (300, 2048, 264), (257, 1100, 264), (129, 520, 1536), (70, 264, 2048), (513, 1031, 1029)])
+def test_contractions_in_pieces(cuda, shape, dt):
+    N, K, F = shape
+    case = gated_case(N, K, F, dt, "silu", True)
+    kept = _lib.lib().tgt_gated_linear_kept_bytes(N, K, F, _lib.DTYPE_F32 if dt == F32 else _lib.DTYPE_BF16, 3)
+    check_gated(*case, "silu", run_gated(*case, "silu"), kept=kept > 0)
+    case = linear_case(N, K, F, dt, True, True)
+    check_linear(*case, None, run_linear(*case, None))
+    x, w, b, r, _ = case
+    wide = torch.empty(F * K + 1, device="cuda", dtype=dt)
+    odd = wide[1:].view(F, K)
+    odd.copy_(w)
+    with torch.no_grad():
+        for weight in (w, odd):
+            check_linear(x, w, b, r, None, "gelu", {"y": T.linear_act(x, weight, b, "gelu", r)})
+
+
 def test_kept_or_formed_again(cuda):
     """The C entry points take both ways at any size: kept values are the products rounded to the type, and the gradients of either way agree with the formula."""
     L = _lib.lib()
@@ -202,7 +222,9 @@ def test_kept_or_formed_again(cuda):
             for keep in (False, True):
                 kept, h = torch.empty(N, 2 * F, device="cuda", dtype=dt), torch.empty(N, F, device="cuda", dtype=dt)
                 kp = kept.data_ptr() if keep else None
-                assert L.tgt_gated_linear_fwd(*P, N, K, F, code, 3, h.data_ptr(), kp, st) == 0
+                nbytes = L.tgt_gated_linear_fwd_workspace_bytes(N, K, F, code)
+                ws = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+                assert L.tgt_gated_linear_fwd(*P, N, K, F, code, 3, h.data_ptr(), kp, ws.data_ptr(), nbytes, st) == 0
                 nbytes = L.tgt_gated_linear_bwd_workspace_bytes(N, K, F, code)
                 ws = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
                 outs = {"h": h, "x": torch.empty_like(x), "wg": torch.empty_like(wg), "wu": torch.empty_like(wu), "bg": torch.empty_like(bg), "bu": torch.empty_like(bu)}
@@ -463,7 +485,7 @@ def test_quantize_rows_is_exact(cuda, dt):
 # ---- operands in 8 bits -------------------------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("out", [F32, BF16])
-@pytest.mark.parametrize("shape", [(1, 16, 1), (1, 1024, 96), (7, 64, 33), (17, 48, 130), (130, 128, 64), (300, 272, 140), (64, 4096, 100)])
+@pytest.mark.parametrize("shape", [(1, 16, 1), (1, 1024, 96), (7, 64, 33), (17, 48, 130), (130, 128, 64), (300, 272, 140), (64, 4096, 100), (200, 4096, 130), (300, 1040, 520), (65, 2048, 264)])
 def test_products_in_8_bits(cuda, out, shape):
     N, K, F = shape
     g = torch.Generator().manual_seed(K + F)

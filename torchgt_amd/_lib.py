@@ -116,14 +116,18 @@ SIGNATURES = {
     "tgt_embedding_sum_bwd_workspace_bytes": (_i64, [_i32, _i32]),
     "tgt_embedding_sum_bwd": (_i32, [_vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _i64, _vp]),
     "tgt_gen_edge_input": (_i32, [_vp, _vp, _i32, _i32, _vp, _i32, _i32, _i32, _vp, _vp]),
-    "tgt_gated_linear_fwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _vp]),
+    "tgt_gated_linear_fwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _i64, _vp]),
+    "tgt_gated_linear_fwd_workspace_bytes": (_i64, [_i64, _i32, _i32, _i32]),
+    "tgt_gated_linear_8bit_workspace_bytes": (_i64, [_i64, _i32, _i32]),
     "tgt_gated_linear_kept_bytes": (_i64, [_i64, _i32, _i32, _i32, _i32]),
-    "tgt_gated_linear_8bit_fwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _vp]),
+    "tgt_gated_linear_8bit_fwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _i64, _vp]),
     "tgt_gated_linear_bwd_workspace_bytes": (_i64, [_i64, _i32, _i32, _i32]),
     "tgt_gated_linear_bwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
-    "tgt_linear_epilogue_fwd": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _vp]),
+    "tgt_linear_epilogue_fwd": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _i64, _vp]),
+    "tgt_linear_epilogue_fwd_workspace_bytes": (_i64, [_i64, _i32, _i32, _i32]),
+    "tgt_linear_epilogue_8bit_workspace_bytes": (_i64, [_i64, _i32, _i32]),
     "tgt_linear_epilogue_kept_bytes": (_i64, [_i64, _i32, _i32, _i32, _i32]),
-    "tgt_linear_epilogue_8bit_fwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _vp]),
+    "tgt_linear_epilogue_8bit_fwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _i64, _vp]),
     "tgt_linear_epilogue_bwd_workspace_bytes": (_i64, [_i64, _i32, _i32, _i32, _i32]),
     "tgt_linear_epilogue_bwd": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
     "tgt_add_rms_norm_fwd": (_i32, [_vp, _vp, _vp, _i64, _i32, _c.c_float, _i32, _vp, _vp, _vp, _vp]),

@@ -71,6 +71,7 @@ struct Args {
     int64_t out_ld;
     int64_t q_first;
     float* partial;            // kWeightGrad with more than one split: [splits][q_count][p_count]
+    f32x4* sums;               // the other forms with more than one split: [splits][tiles][waves][pieces of a wave][64 lanes], as the waves hold them
     int act;
     unsigned p_tiles, q_tiles;
 };
@@ -275,8 +276,8 @@ template <int COLS, int ROWS, int WP_, int WQ_> struct Shape {
     static constexpr int kCols = COLS, kRows = ROWS, WP = WP_, WQ = WQ_, kThreads = 64 * WP * WQ;
     static constexpr int FP = COLS / WP / 16, FQ = ROWS / WQ / 16;      // 16 x 16 pieces of a wave
     // which 16 columns / rows of the tile a wave's piece is
-    static __device__ __forceinline__ int p_piece(int wave, int i) { return wave % WP * FP + i; }
-    static __device__ __forceinline__ int q_piece(int wave, int j) { return wave / WP * FQ + j; }
+    static constexpr __host__ __device__ __forceinline__ int p_piece(int wave, int i) { return wave % WP * FP + i; }
+    static constexpr __host__ __device__ __forceinline__ int q_piece(int wave, int j) { return wave / WP * FQ + j; }
 };
 
 // acc[i][j]: columns 16 i .., rows 16 j .. of the wave's part of the tile.  lds: STAGES times the tiles' bytes.
@@ -388,6 +389,19 @@ __device__ __forceinline__ void product(const Args& a, int64_t p0, int64_t q0, i
     }
 }
 
+// One split's sums of a tile, pieces outside the result left out
+template <typename S>
+__device__ __forceinline__ void put_sums(const Args& a, int by, int64_t p0, int64_t q0, unsigned split, const f32x4 (&acc)[S::FP][S::FQ]) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t tile = ((int64_t)split * a.q_tiles + q0 / S::kRows) * a.p_tiles + p0 / (S::kCols / by);
+    f32x4* to = a.sums + (tile * (S::kThreads / 64) + wave) * (S::FP * S::FQ * 64) + lane;
+#pragma unroll
+    for (int i = 0; i < S::FP; ++i)
+#pragma unroll
+        for (int j = 0; j < S::FQ; ++j)
+            if (p0 + S::p_piece(wave, i) / by * 16 < a.p_count && q0 + S::q_piece(wave, j) * 16 < a.q_count) to[(i * S::FQ + j) * 64] = acc[i][j];
+}
+
 // Workgroup -> tile and split.  Consecutive workgroups go to the eight XCDs in turn, each with an L2 of its own: XCD x takes the places from x / 8 of
 // the way on; one split after the other, of a split eight rows of tiles at a time, column by column, so that the tiles that run there together
 // share both operands.
@@ -422,8 +436,8 @@ template <int PH_> struct Wide {
     static constexpr int PH = PH_, kCols = 128 * PH, kRows = 256, kThreads = 512, FP = 4 * PH, FQ = 4;
     static constexpr int kHalf = 128 * 128, kOperand = PH * kHalf, kStage = kOperand + 2 * kHalf, kStages = PH == 2 ? 2 : 3, kLds = kStages * kStage;
     // waves 0-3 and 4-7 have 64 columns of each half of P, a wave 32 rows of each half of Q
-    static __device__ __forceinline__ int p_piece(int wave, int i) { return (i >> 2) * 8 + (wave >> 2) * 4 + (i & 3); }
-    static __device__ __forceinline__ int q_piece(int wave, int j) { return (j >> 1) * 8 + (wave & 3) * 2 + (j & 1); }
+    static constexpr __host__ __device__ __forceinline__ int p_piece(int wave, int i) { return (i >> 2) * 8 + (wave >> 2) * 4 + (i & 3); }
+    static constexpr __host__ __device__ __forceinline__ int q_piece(int wave, int j) { return (j >> 1) * 8 + (wave & 3) * 2 + (j & 1); }
 };
 
 // 16 bytes for each lane, from an address of the wave and 32 bits of the lane's, to 1 KB of LDS at byte `at`.  A buffer instruction: with a global one the
@@ -498,7 +512,10 @@ template <typename T, int FORM, bool TWO, typename S> struct Stream {
         if constexpr (FORM == kInputGrad && TWO) {
             cross = reinterpret_cast<const char*>(a.P[1]) - reinterpret_cast<const char*>(a.P[0]) - a.K_first * a.p_ld * (int64_t)sizeof(T);
 #pragma unroll
-            for (int h = 0; h < S::PH; ++h) until[h] = a.K_first / Kind<T>::kStep;
+            for (int h = 0; h < S::PH; ++h) {
+                until[h] = (a.K_first - k0) / Kind<T>::kStep;
+                if (k0 > a.K_first) P.base[h] += cross;      // (a split that starts in the second: the steps until then stay below zero)
+            }
         }
     }
     __device__ __forceinline__ void ask_p(int half, char* stage) {

@@ -224,6 +224,9 @@ __global__ __launch_bounds__(S::kThreads) void k_product(const Args a, const uns
     const int64_t k0 = (int64_t)split * a.K_each, k1 = k0 + a.K_each < a.K ? k0 + a.K_each : a.K;
     f32x4 acc[S::FP][S::FQ];
     product<T, FORM, TWO, ALIGNED, S, STAGES>(a, p0, q0, k0, k1, lds, acc);
+    if constexpr (FORM != kWeightGrad && !GRAD) {
+        if (a.sums) return put_sums<S>(a, FORM == kForward && TWO ? 2 : 1, p0, q0, split, acc);
+    }
     epilogue<T, O, FORM, TWO, GRAD, S>(a, p0, q0, split, acc);
 }
 
@@ -264,8 +267,43 @@ __global__ __launch_bounds__(S::kThreads, 2) void k_wide(const Args a, const uns
         if (done < now.k1) stream.rest(a, now.p0, now.q0, done, now.k1, lds, acc);
         more = find(next);
         if (more) stream.ask_first(lds, next.steps);
+        if constexpr (FORM != kWeightGrad && !GRAD) {
+            if (a.sums) {
+                put_sums<S>(a, FORM == kForward && TWO ? 2 : 1, now.p0, now.q0, now.split, acc);
+                continue;
+            }
+        }
         epilogue<T, O, FORM, TWO, GRAD, S>(a, now.p0, now.q0, now.split, acc);
     }
+}
+
+// The splits' sums of a tile S, added in their order, and what becomes of them: two pieces of columns and one of rows of each wave to a workgroup.
+template <typename S> struct Part {
+    static constexpr int kThreads = S::kThreads, FP = 2, FQ = 1, kLast = S::kThreads / 64 - 1;
+    static constexpr int kParts = S::FQ * S::FP / 2;
+    static __device__ __forceinline__ int p_piece(int wave, int i) { return S::p_piece(wave, i); }
+    static __device__ __forceinline__ int q_piece(int wave, int) { return S::q_piece(wave, 0); }
+    static constexpr int kCols = (S::p_piece(kLast, 1) + 1) * 16, kRows = (S::q_piece(kLast, 0) + 1) * 16;      // what they span
+};
+template <typename T, typename O, int FORM, bool TWO, typename S>
+__global__ __launch_bounds__(S::kThreads) void k_join(const Args a, const unsigned splits) {
+    constexpr int kBy = FORM == kForward && TWO ? 2 : 1;
+    const unsigned tile = blockIdx.x / Part<S>::kParts, part = blockIdx.x % Part<S>::kParts, j = part % S::FQ, i = part / S::FQ * 2;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t p0 = (int64_t)(tile % a.p_tiles) * (S::kCols / kBy) + S::p_piece(0, i) / kBy * 16, q0 = (int64_t)(tile / a.p_tiles) * S::kRows + S::q_piece(0, j) * 16;
+    if (p0 + S::p_piece(wave, 0) / kBy * 16 >= a.p_count || q0 + S::q_piece(wave, 0) * 16 >= a.q_count) return;
+    const bool both = p0 + S::p_piece(wave, 1) / kBy * 16 < a.p_count;
+    const int64_t each = (int64_t)a.p_tiles * a.q_tiles * S::kThreads * (S::FP * S::FQ);
+    const f32x4* from = a.sums + ((int64_t)tile * (S::kThreads / 64) + wave) * (S::FP * S::FQ * 64) + (i * S::FQ + j) * 64 + lane;
+    const int second = both ? S::FQ * 64 : 0;
+    f32x4 total[2][1] = {{f32x4{0.f, 0.f, 0.f, 0.f}}, {f32x4{0.f, 0.f, 0.f, 0.f}}};
+#pragma unroll 4
+    for (unsigned s = 0; s < splits; ++s) {
+        const f32x4 x = from[s * each], y = from[s * each + second];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { total[0][0][e] += x[e]; total[1][0][e] += y[e]; }
+    }
+    epilogue<T, O, FORM, TWO, false, Part<S>>(a, p0, q0, 0, total);
 }
 
 // Products of few rows (up to 16 NQ): bound by the weights' bytes.  A workgroup has 16 columns of the result, its waves a share of the contraction each, operands go
@@ -419,18 +457,19 @@ __global__ __launch_bounds__(256) void k_kept_grad(const O* __restrict__ kept, c
     for (int w = 0; w < NW; ++w)
 #pragma unroll
         for (int e = 0; e < VE; ++e) sums[w][e] = 0.f;
-    for (int64_t r = r0; r < r1; r += 2) {      // two rows in flight
-        Some in[2][NW + 1];
-        const int n = r + 1 < r1 ? 2 : 1;
+    constexpr int U = 4;      // rows in flight
+    for (int64_t r = r0; r < r1; r += U) {
+        Some in[U][NW + 1];
+        const int n = r1 - r < U ? (int)(r1 - r) : U;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < U; ++i) {
             const int64_t row = i < n ? r + i : r;
 #pragma unroll
             for (int w = 0; w < NW; ++w) in[i][w] = *reinterpret_cast<const Some*>(kept + (row * NW + w) * F + c);
             in[i][NW] = *reinterpret_cast<const Some*>(dy + row * F + c);
         }
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < U; ++i) {
             if (i >= n) break;
             Some out[NW];
 #pragma unroll
@@ -489,6 +528,13 @@ __global__ __launch_bounds__(256) void k_zero(uint16_t* __restrict__ p, int64_t 
 
 using Square = Shape<128, 128, 2, 2>;
 
+template <typename T, typename O, int FORM, bool TWO, typename S> int join(const Args& a, int splits, hipStream_t st) {
+    if (!a.sums) return TGT_OK;
+    hipLaunchKernelGGL((k_join<T, O, FORM, TWO, S>), dim3(a.p_tiles * a.q_tiles * Part<S>::kParts), dim3(S::kThreads), 0, st, a, (unsigned)splits);
+    TGT_HIP_CHECK(hipGetLastError());
+    return TGT_OK;
+}
+
 template <typename T, typename O, int FORM, bool TWO, bool GRAD, bool ALIGNED, typename S, int STAGES>
 int launch(Args a, int splits, hipStream_t st) {
     constexpr int kCols = FORM == kForward && TWO ? S::kCols / 2 : S::kCols;
@@ -505,6 +551,7 @@ int launch(Args a, int splits, hipStream_t st) {
     }
     hipLaunchKernelGGL(kernel, dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(S::kThreads), kLds, st, a, (unsigned)splits);
     TGT_HIP_CHECK(hipGetLastError());
+    if constexpr (FORM != kWeightGrad && !GRAD) return join<T, O, FORM, TWO, S>(a, splits, st);
     return TGT_OK;
 }
 
@@ -522,6 +569,7 @@ int launch_wide(Args a, int splits, hipStream_t st) {
     const unsigned grid = (unsigned)std::min<int64_t>(places, num_cus() / 8 * 8);
     hipLaunchKernelGGL(kernel, dim3(grid), dim3(S::kThreads), S::kLds, st, a, (unsigned)places, (unsigned)splits);
     TGT_HIP_CHECK(hipGetLastError());
+    if constexpr (FORM != kWeightGrad && !GRAD) return join<T, O, FORM, TWO, S>(a, splits, st);
     return TGT_OK;
 }
 
@@ -540,10 +588,35 @@ template <typename T, typename O, bool TWO, int NQ, bool ALIGNED> int launch_few
     TGT_HIP_CHECK(hipGetLastError());
     return TGT_OK;
 }
-// Tiles of `cols` x 256 that keep the CUs busy
-bool wide_enough(const Args& a, int cols, int splits) {
-    const int64_t tiles = (a.p_count + cols - 1) / cols * ((a.q_count + 255) / 256) * splits;
-    return tiles >= 200 && a.K >= 256 && a.p_ld < (1 << 21) && a.q_ld < (1 << 21);
+// How a product is cut: tiles of 128 x 128 (halves 0) or 256 rows x 128 or 256 columns (kernels for 16- and 8-bit operands, aligned rows that 32-bit offsets
+// reach, K >= 256), and splits of the contraction where there are fewer tiles than CUs, whose sums are joined by a kernel of their own.  What is taken is what
+// takes least by this account, in us, fitted to measurements of each kernel at K 256 to 8192 and 64 to 1024 tiles:
+struct Way { int halves, splits; int64_t K_each, bytes; };
+template <typename T> Way way_of(int64_t p_count, int64_t q_count, int64_t K, int by, bool wide, bool cut) {
+    constexpr int kSize = sizeof(T);
+    static constexpr double kFixed[3] = {kSize == 4 ? 4. : 5., 8.5, 14.}, kStep[3] = {kSize == 4 ? 2.8 : kSize == 2 ? 1.2 : 1.1, .85, 1.44};
+    const int64_t cus = num_cus(), steps = (K + Kind<T>::kStep - 1) / Kind<T>::kStep;
+    Way best{};
+    double least = 1e300;
+    for (int h = 0; h <= (wide ? kSize == 1 ? 1 : 2 : 0); ++h) {      // (8-bit operands beside 128 sums: no registers, and reloads from scratch wait for all loads)
+        const int64_t cols = (h == 2 ? 256 : 128) / by, rows = h ? 256 : 128, tiles = (p_count + cols - 1) / cols * ((q_count + rows - 1) / rows);
+        const int64_t most = cut && h < 2 ? std::min(cus / tiles, steps / 2) : 1;
+        for (int64_t s = 1; s == 1 || s <= most; ++s) {
+            const int64_t each = (steps + s - 1) / s, bytes = s > 1 ? s * tiles * rows * 128 * 4 : 0;
+            if ((steps + each - 1) / each != s) continue;
+            const double us = (tiles * s + cus - 1) / cus * (kFixed[h] + each * kStep[h]) + (s > 1 ? 4. + bytes * .4e-6 : 0.);
+            if (us < least) { least = us; best = Way{h, (int)s, each * Kind<T>::kStep, bytes}; }
+        }
+    }
+    return best;
+}
+bool wide_rows(const Args& a) { return a.K >= 256 && a.p_ld < (1 << 21) && a.q_ld < (1 << 21); }
+// a tile of one half takes 0.59 of the time of one with two
+int wide_halves(const Args& a, int cols, int splits) {
+    if (!wide_rows(a)) return 0;
+    const int64_t high = (a.q_count + 255) / 256 * splits, cus = num_cus(), one = (a.p_count + cols - 1) / cols * high, two = (a.p_count + 2 * cols - 1) / (2 * cols) * high;
+    if (one < cus * 3 / 4) return 0;
+    return 100 * ((two + cus - 1) / cus) <= 59 * ((one + cus - 1) / cus) ? 2 : 1;
 }
 
 bool aligned16(const void* p, int64_t ld, int size) { return ((uintptr_t)p & 15) == 0 && ld * size % 16 == 0; }
@@ -551,12 +624,28 @@ bool aligned16(const void* p, int64_t ld, int size) { return ((uintptr_t)p & 15)
 }  // namespace
 
 // One product in the form asked for; TWO: a.P[1] is given
-template <typename T, typename O> int product_forward(const Args& a, bool grad, hipStream_t st);
-template <typename T> int product_input_grad(const Args& a, hipStream_t st);
+struct Room { void* p; int64_t bytes; };      // for the sums of splits
+template <typename T, typename O> int product_forward(Args a, bool grad, Room room, hipStream_t st);
+template <typename T> int product_input_grad(Args a, Room room, hipStream_t st);
 template <typename T> int product_weight_grad(const Args& a, int splits, hipStream_t st);
 
+// Bytes that the sums of splits take, whatever the operands' alignment
+template <typename T> int64_t room_of(int64_t p_count, int64_t q_count, int64_t K, int by) {
+    return std::max(way_of<T>(p_count, q_count, K, by, false, true).bytes, way_of<T>(p_count, q_count, K, by, sizeof(T) < 4 && K >= 256, true).bytes);
+}
+
 #if TGT_GATED_PART > 0
-template <typename T, typename O> int product_forward(const Args& a, bool grad, hipStream_t st) {
+int take(Args& a, const Way& way, const Room& room) {
+    a.K_each = way.K_each;
+    if (!way.bytes) return TGT_OK;
+    if (!room.p || room.bytes < way.bytes || ((uintptr_t)room.p & 15)) {
+        set_error("torchgt: a product's workspace of %lld bytes (16-byte aligned) needed, got %lld", (long long)way.bytes, (long long)room.bytes);
+        return TGT_ERR_WORKSPACE;
+    }
+    a.sums = reinterpret_cast<f32x4*>(room.p);
+    return TGT_OK;
+}
+template <typename T, typename O> int product_forward(Args a, bool grad, Room room, hipStream_t st) {
     constexpr int kStages = sizeof(T) == 4 ? 1 : 2;
     const bool two = a.P[1] != nullptr;
     const bool al = aligned16(a.Q, a.q_ld, sizeof(T)) && aligned16(a.P[0], a.p_ld, sizeof(T)) && (!two || aligned16(a.P[1], a.p_ld, sizeof(T)));
@@ -566,16 +655,15 @@ template <typename T, typename O> int product_forward(const Args& a, bool grad, 
         X(false, 1, false); X(true, 1, false); X(false, 2, false); X(true, 2, false); X(false, 4, false); X(true, 4, false);
 #undef X
     }
+    const Way way = way_of<T>(a.p_count, a.q_count, a.K, two ? 2 : 1, sizeof(T) < 4 && al && wide_rows(a), !grad);
+    if (const int rc = take(a, way, room)) return rc;
     if constexpr (sizeof(T) < 4) {
-        constexpr int PH = sizeof(T) == 1 ? 1 : 2;
-        if (al && wide_enough(a, (two ? 64 : 128) * PH, 1)) {
-#define X(TWO, GRAD) if (two == TWO && grad == GRAD) return launch_wide<T, O, kForward, TWO, GRAD, Wide<PH>>(a, 1, st)
-            X(false, false); X(true, false);
-            if constexpr (sizeof(T) > 1) { X(false, true); X(true, true); }
+#define X(TWO, GRAD, PH) if (two == TWO && grad == GRAD && way.halves == PH) return launch_wide<T, O, kForward, TWO, GRAD, Wide<PH>>(a, way.splits, st)
+        X(false, false, 1); X(true, false, 1);
+        if constexpr (sizeof(T) > 1) { X(false, false, 2); X(true, false, 2); X(false, true, 1); X(true, true, 1); X(false, true, 2); X(true, true, 2); }
 #undef X
-        }
     }
-#define X(TWO, GRAD, AL) if (two == TWO && grad == GRAD && al == AL) return launch<T, O, kForward, TWO, GRAD, AL, Square, kStages>(a, 1, st)
+#define X(TWO, GRAD, AL) if (two == TWO && grad == GRAD && al == AL) return launch<T, O, kForward, TWO, GRAD, AL, Square, kStages>(a, way.splits, st)
     X(false, false, true); X(true, false, true); X(false, false, false); X(true, false, false);
     if constexpr (sizeof(T) > 1) { X(false, true, true); X(true, true, true); X(false, true, false); X(true, true, false); }
 #undef X
@@ -583,17 +671,18 @@ template <typename T, typename O> int product_forward(const Args& a, bool grad, 
 }
 #endif
 #if TGT_GATED_PART == 1 || TGT_GATED_PART == 2
-template <typename T> int product_input_grad(const Args& a, hipStream_t st) {
+template <typename T> int product_input_grad(Args a, Room room, hipStream_t st) {
     constexpr int kStages = sizeof(T) == 4 ? 1 : 2;
     const bool two = a.P[1] != nullptr;
     const bool al = aligned16(a.Q, a.q_ld, sizeof(T)) && aligned16(a.P[0], a.p_ld, sizeof(T)) && (!two || aligned16(a.P[1], a.p_ld, sizeof(T)));
+    const Way way = way_of<T>(a.p_count, a.q_count, a.K, 1, sizeof(T) < 4 && al && wide_rows(a) && a.p_count % 8 == 0 && (!two || a.K_first % Kind<T>::kStep == 0), true);
+    if (const int rc = take(a, way, room)) return rc;
     if constexpr (sizeof(T) < 4) {
-        if (al && a.p_count % 8 == 0 && (!two || a.K_first % Kind<T>::kStep == 0) && wide_enough(a, 256, 1)) {
-            if (two) return launch_wide<T, T, kInputGrad, true, false, Wide<2>>(a, 1, st);
-            return launch_wide<T, T, kInputGrad, false, false, Wide<2>>(a, 1, st);
-        }
+#define X(TWO, PH) if (two == TWO && way.halves == PH) return launch_wide<T, T, kInputGrad, TWO, false, Wide<PH>>(a, way.splits, st)
+        X(false, 1); X(true, 1); X(false, 2); X(true, 2);
+#undef X
     }
-#define X(TWO, AL) if (two == TWO && al == AL) return launch<T, T, kInputGrad, TWO, false, AL, Square, kStages>(a, 1, st)
+#define X(TWO, AL) if (two == TWO && al == AL) return launch<T, T, kInputGrad, TWO, false, AL, Square, kStages>(a, way.splits, st)
     X(false, true); X(true, true); X(false, false); X(true, false);
 #undef X
     return TGT_ERR_INVALID_ARG;
@@ -602,26 +691,25 @@ template <typename T> int product_weight_grad(const Args& a, int splits, hipStre
     constexpr int kStages = sizeof(T) == 4 ? 1 : 2;
     const bool al = aligned16(a.Q, a.q_ld, sizeof(T)) && aligned16(a.P[0], a.p_ld, sizeof(T));
     if constexpr (sizeof(T) < 4) {
-        if (al && a.p_count % 8 == 0 && a.q_count % 8 == 0) {
-            if (wide_enough(a, 256, splits)) return launch_wide<T, T, kWeightGrad, false, false, Wide<2>>(a, splits, st);
-            if (wide_enough(a, 128, splits)) return launch_wide<T, T, kWeightGrad, false, false, Wide<1>>(a, splits, st);
-        }
+        const int halves = al && a.p_count % 8 == 0 && a.q_count % 8 == 0 ? wide_halves(a, 128, splits) : 0;
+        if (halves == 2) return launch_wide<T, T, kWeightGrad, false, false, Wide<2>>(a, splits, st);
+        if (halves == 1) return launch_wide<T, T, kWeightGrad, false, false, Wide<1>>(a, splits, st);
     }
     if (al) return launch<T, T, kWeightGrad, false, false, true, Square, kStages>(a, splits, st);
     return launch<T, T, kWeightGrad, false, false, false, Square, kStages>(a, splits, st);
 }
 #endif
 #if TGT_GATED_PART == 1
-template int product_forward<b16, b16>(const Args&, bool, hipStream_t);
-template int product_input_grad<b16>(const Args&, hipStream_t);
+template int product_forward<b16, b16>(Args, bool, Room, hipStream_t);
+template int product_input_grad<b16>(Args, Room, hipStream_t);
 template int product_weight_grad<b16>(const Args&, int, hipStream_t);
 #elif TGT_GATED_PART == 2
-template int product_forward<float, float>(const Args&, bool, hipStream_t);
-template int product_input_grad<float>(const Args&, hipStream_t);
+template int product_forward<float, float>(Args, bool, Room, hipStream_t);
+template int product_input_grad<float>(Args, Room, hipStream_t);
 template int product_weight_grad<float>(const Args&, int, hipStream_t);
 #elif TGT_GATED_PART == 3
-template int product_forward<e4m3, b16>(const Args&, bool, hipStream_t);
-template int product_forward<e4m3, float>(const Args&, bool, hipStream_t);
+template int product_forward<e4m3, b16>(Args, bool, Room, hipStream_t);
+template int product_forward<e4m3, float>(Args, bool, Room, hipStream_t);
 #else
 
 namespace {
@@ -694,7 +782,7 @@ NarrowArgs narrow_args(const Call& c, const void* more) {
 // comments on k_kept_grad; about 4 K / 1.2e15 + 2e-12 s a value against 3e-12.
 bool keeps(const Call& c) { return needs_du(c.n, c.act) && c.N > 64 && !narrow(c) && c.K >= (c.dtype == TGT_DTYPE_F32 ? 128 : 512); }
 
-int forward(const Call& c, const void* residual, void* out, void* kept, hipStream_t st) {
+int forward(const Call& c, const void* residual, void* out, void* kept, Room room, hipStream_t st) {
     int rc = check_call(c);
     if (rc != TGT_OK || c.N == 0) return rc;
     if (!out) { set_error("%s: null pointer", c.who); return TGT_ERR_INVALID_ARG; }
@@ -709,10 +797,10 @@ int forward(const Call& c, const void* residual, void* out, void* kept, hipStrea
     a.out[0] = out;
     a.kept = kept;
     KernelTimer t(KS_LINEAR_FWD, st);
-    return c.dtype == TGT_DTYPE_F32 ? product_forward<float, float>(a, false, st) : product_forward<b16, b16>(a, false, st);
+    return c.dtype == TGT_DTYPE_F32 ? product_forward<float, float>(a, false, room, st) : product_forward<b16, b16>(a, false, room, st);
 }
 
-int forward_8bit(const Call& c, const float* x_scales, const float* s0, const float* s1, const void* residual, void* out, hipStream_t st) {
+int forward_8bit(const Call& c, const float* x_scales, const float* s0, const float* s1, const void* residual, void* out, Room room, hipStream_t st) {
     int rc = check_call(c);
     if (rc != TGT_OK) return rc;
     if (c.K % 16) {
@@ -727,13 +815,13 @@ int forward_8bit(const Call& c, const float* x_scales, const float* s0, const fl
     a.residual = residual;
     a.out[0] = out;
     KernelTimer t(KS_LINEAR_FWD, st);
-    return c.dtype == TGT_DTYPE_F32 ? product_forward<e4m3, float>(a, false, st) : product_forward<e4m3, b16>(a, false, st);
+    return c.dtype == TGT_DTYPE_F32 ? product_forward<e4m3, float>(a, false, room, st) : product_forward<e4m3, b16>(a, false, room, st);
 }
 
 // How the backward lays out its workspace, and how it cuts the nodes
 struct Plan {
-    int64_t du_bytes, bytes, K_each, rows_each;
-    int splits, shares;
+    int64_t du_bytes, between, bytes, K_each, rows_each;
+    int splits, shares, kept_shares;
 };
 int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
 Plan plan_of(int n, int64_t N, int K, int F, int dtype, int act) {
@@ -748,7 +836,10 @@ Plan plan_of(int n, int64_t N, int K, int F, int dtype, int act) {
     p.splits = N > 0 ? (int)((N + p.K_each - 1) / p.K_each) : 1;
     p.shares = (int)std::max<int64_t>(1, std::min<int64_t>(512, (N + 31) / 32));
     p.rows_each = (N + p.shares - 1) / p.shares;
-    p.bytes = p.du_bytes + (p.splits > 1 ? up16((int64_t)p.splits * cols * K * 4) : 0) + up16((int64_t)p.shares * cols * 4);
+    p.kept_shares = (int)std::max<int64_t>(1, std::min<int64_t>(512, (N + 7) / 8));      // (their rows are in flight together: latency counts before bandwidth)
+    // one after the other: the sums of dx's splits, those of the weights' gradients
+    p.between = std::max(p.splits > 1 ? up16((int64_t)p.splits * cols * K * 4) : 0, dtype == TGT_DTYPE_F32 ? room_of<float>(K, N, cols, 1) : room_of<b16>(K, N, cols, 1));
+    p.bytes = p.du_bytes + p.between + up16((int64_t)p.kept_shares * cols * 4);
     return p;
 }
 
@@ -831,11 +922,11 @@ int backward(const Call& c, const void* kept, const void* dy, void* dx, void* co
     char* ws = (char*)workspace;
     if (!kept && narrow_backward(c, dy)) return backward_narrow(c, dy, dx, dW, db, ws, st);
     const void* du = dy;
-    float* sums = (float*)(ws + p.bytes - up16((int64_t)p.shares * cols * 4));
+    float* sums = (float*)(ws + p.bytes - up16((int64_t)p.kept_shares * cols * 4));
     if (p.du_bytes && kept) {
         KernelTimer t(KS_GELU, st);
-        if (f32) launch_kept_grad<float>(kept, dy, c.n, c.N, c.F, p.rows_each, p.shares, c.act, ws, want_b ? sums : nullptr, st);
-        else launch_kept_grad<b16>(kept, dy, c.n, c.N, c.F, p.rows_each, p.shares, c.act, ws, want_b ? sums : nullptr, st);
+        if (f32) launch_kept_grad<float>(kept, dy, c.n, c.N, c.F, (c.N + p.kept_shares - 1) / p.kept_shares, p.kept_shares, c.act, ws, want_b ? sums : nullptr, st);
+        else launch_kept_grad<b16>(kept, dy, c.n, c.N, c.F, (c.N + p.kept_shares - 1) / p.kept_shares, p.kept_shares, c.act, ws, want_b ? sums : nullptr, st);
         TGT_HIP_CHECK(hipGetLastError());
         du = ws;
     } else if (p.du_bytes) {
@@ -845,7 +936,7 @@ int backward(const Call& c, const void* kept, const void* dy, void* dx, void* co
         a.out[1] = c.n == 2 ? ws + c.F * size : nullptr;
         a.out_ld = cols;
         KernelTimer t(KS_LINEAR_FWD, st);
-        rc = f32 ? product_forward<float, float>(a, true, st) : product_forward<b16, b16>(a, true, st);
+        rc = f32 ? product_forward<float, float>(a, true, Room{}, st) : product_forward<b16, b16>(a, true, Room{}, st);
         if (rc != TGT_OK) return rc;
         du = ws;
     }
@@ -859,7 +950,8 @@ int backward(const Call& c, const void* kept, const void* dy, void* dx, void* co
         a.out[0] = dx;
         a.out_ld = c.K;
         KernelTimer t(KS_LINEAR_DX, st);
-        rc = f32 ? product_input_grad<float>(a, st) : product_input_grad<b16>(a, st);
+        const Room room{ws + p.du_bytes, p.between};
+        rc = f32 ? product_input_grad<float>(a, room, st) : product_input_grad<b16>(a, room, st);
         if (rc != TGT_OK) return rc;
     }
     char* after = ws + p.du_bytes;
@@ -900,7 +992,7 @@ int backward(const Call& c, const void* kept, const void* dy, void* dx, void* co
             TGT_HIP_CHECK(hipGetLastError());
         }
         tgt_reduce_desc r{};
-        r.partial = sums; r.workers = p.shares; r.n = (int)cols; r.n_out = c.n;
+        r.partial = sums; r.workers = p.du_bytes && kept ? p.kept_shares : p.shares; r.n = (int)cols; r.n_out = c.n;
         r.out[0] = db[0]; r.begin[0] = 0;
         if (c.n == 2) { r.out[1] = db[1]; r.begin[1] = c.F; }
         return reduce_partials(&r, 1, c.dtype, st);
@@ -912,6 +1004,11 @@ int64_t kept_bytes_of(int n, int64_t N, int K, int F, int dtype, int act) {
     if (N < 0 || K < 1 || F < 1 || (dtype != TGT_DTYPE_F32 && dtype != TGT_DTYPE_BF16)) return -1;
     const Call c{"", nullptr, {nullptr, nullptr}, {nullptr, nullptr}, n, N, K, F, dtype, act};
     return keeps(c) ? N * n * F * (dtype == TGT_DTYPE_F32 ? 4 : 2) : 0;
+}
+int64_t fwd_bytes_of(int n, int64_t N, int K, int F, int dtype, bool bits8) {
+    if (N < 0 || K < 1 || F < 1 || (dtype != TGT_DTYPE_F32 && dtype != TGT_DTYPE_BF16)) return -1;
+    if (N <= 64) return 0;
+    return bits8 ? room_of<e4m3>(F, N, K, n) : dtype == TGT_DTYPE_F32 ? room_of<float>(F, N, K, n) : room_of<b16>(F, N, K, n);
 }
 int64_t workspace_bytes_of(int n, int64_t N, int K, int F, int dtype, int act) {
     if (N < 0 || K < 1 || F < 1 || (dtype != TGT_DTYPE_F32 && dtype != TGT_DTYPE_BF16)) return -1;
@@ -930,17 +1027,24 @@ int64_t workspace_bytes_of(int n, int64_t N, int K, int F, int dtype, int act) {
 extern "C" {
 
 int tgt_gated_linear_fwd(const void* d_x, const void* d_Wg, const void* d_Wu, const void* d_bg, const void* d_bu, int64_t N, int in_features, int out_features,
-                         int dtype, int act, void* d_h, void* d_kept, void* stream) {
+                         int dtype, int act, void* d_h, void* d_kept, void* d_workspace, int64_t workspace_bytes, void* stream) {
     const tgt::Call c{"tgt_gated_linear_fwd", d_x, {d_Wg, d_Wu}, {d_bg, d_bu}, 2, N, in_features, out_features, dtype, act};
-    return tgt::forward(c, nullptr, d_h, d_kept, (hipStream_t)stream);
+    return tgt::forward(c, nullptr, d_h, d_kept, {d_workspace, workspace_bytes}, (hipStream_t)stream);
+}
+int64_t tgt_gated_linear_fwd_workspace_bytes(int64_t N, int in_features, int out_features, int dtype) {
+    return tgt::fwd_bytes_of(2, N, in_features, out_features, dtype, false);
+}
+int64_t tgt_gated_linear_8bit_workspace_bytes(int64_t N, int in_features, int out_features) {
+    return tgt::fwd_bytes_of(2, N, in_features, out_features, TGT_DTYPE_F32, true);
 }
 int64_t tgt_gated_linear_kept_bytes(int64_t N, int in_features, int out_features, int dtype, int act) {
     return tgt::kept_bytes_of(2, N, in_features, out_features, dtype, act);
 }
 int tgt_gated_linear_8bit_fwd(const void* d_x, const float* d_x_scales, const void* d_Wg, const float* d_Wg_scales, const void* d_Wu, const float* d_Wu_scales,
-                              const void* d_bg, const void* d_bu, int64_t N, int in_features, int out_features, int dtype, int act, void* d_h, void* stream) {
+                              const void* d_bg, const void* d_bu, int64_t N, int in_features, int out_features, int dtype, int act, void* d_h, void* d_workspace,
+                              int64_t workspace_bytes, void* stream) {
     const tgt::Call c{"tgt_gated_linear_8bit_fwd", d_x, {d_Wg, d_Wu}, {d_bg, d_bu}, 2, N, in_features, out_features, dtype, act};
-    return tgt::forward_8bit(c, d_x_scales, d_Wg_scales, d_Wu_scales, nullptr, d_h, (hipStream_t)stream);
+    return tgt::forward_8bit(c, d_x_scales, d_Wg_scales, d_Wu_scales, nullptr, d_h, {d_workspace, workspace_bytes}, (hipStream_t)stream);
 }
 int64_t tgt_gated_linear_bwd_workspace_bytes(int64_t N, int in_features, int out_features, int dtype) {
     return tgt::workspace_bytes_of(2, N, in_features, out_features, dtype, TGT_ACT_SILU);
@@ -953,17 +1057,24 @@ int tgt_gated_linear_bwd(const void* d_x, const void* d_Wg, const void* d_Wu, co
 }
 
 int tgt_linear_epilogue_fwd(const void* d_x, const void* d_W, const void* d_b, const void* d_residual, int64_t N, int in_features, int out_features, int dtype,
-                            int act, void* d_y, void* d_kept, void* stream) {
+                            int act, void* d_y, void* d_kept, void* d_workspace, int64_t workspace_bytes, void* stream) {
     const tgt::Call c{"tgt_linear_epilogue_fwd", d_x, {d_W, nullptr}, {d_b, nullptr}, 1, N, in_features, out_features, dtype, act};
-    return tgt::forward(c, d_residual, d_y, d_kept, (hipStream_t)stream);
+    return tgt::forward(c, d_residual, d_y, d_kept, {d_workspace, workspace_bytes}, (hipStream_t)stream);
+}
+int64_t tgt_linear_epilogue_fwd_workspace_bytes(int64_t N, int in_features, int out_features, int dtype) {
+    return tgt::fwd_bytes_of(1, N, in_features, out_features, dtype, false);
+}
+int64_t tgt_linear_epilogue_8bit_workspace_bytes(int64_t N, int in_features, int out_features) {
+    return tgt::fwd_bytes_of(1, N, in_features, out_features, TGT_DTYPE_F32, true);
 }
 int64_t tgt_linear_epilogue_kept_bytes(int64_t N, int in_features, int out_features, int dtype, int act) {
     return tgt::kept_bytes_of(1, N, in_features, out_features, dtype, act);
 }
 int tgt_linear_epilogue_8bit_fwd(const void* d_x, const float* d_x_scales, const void* d_W, const float* d_W_scales, const void* d_b, const void* d_residual,
-                                 int64_t N, int in_features, int out_features, int dtype, int act, void* d_y, void* stream) {
+                                 int64_t N, int in_features, int out_features, int dtype, int act, void* d_y, void* d_workspace, int64_t workspace_bytes,
+                                 void* stream) {
     const tgt::Call c{"tgt_linear_epilogue_8bit_fwd", d_x, {d_W, nullptr}, {d_b, nullptr}, 1, N, in_features, out_features, dtype, act};
-    return tgt::forward_8bit(c, d_x_scales, d_W_scales, nullptr, d_residual, d_y, (hipStream_t)stream);
+    return tgt::forward_8bit(c, d_x_scales, d_W_scales, nullptr, d_residual, d_y, {d_workspace, workspace_bytes}, (hipStream_t)stream);
 }
 int64_t tgt_linear_epilogue_bwd_workspace_bytes(int64_t N, int in_features, int out_features, int dtype, int act) {
     return tgt::workspace_bytes_of(1, N, in_features, out_features, dtype, act);

@@ -160,13 +160,18 @@ void check_residual(const Optional& r, const Tensor& x, at::ScalarType type, int
     TORCH_CHECK(r->scalar_type() == type && r->sizes() == at::IntArrayRef(with_last(x, F)), op, ": residual must be ", type, " of the result's shape");
 }
 
+Tensor room(int64_t bytes, const Tensor& x) { return bytes > 0 ? at::empty({bytes}, x.options().dtype(at::kByte)) : Tensor(); }
+void* at_of(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
 // kept: null, or where to put what the forward keeps for a backward
 Tensor gated_forward(const Tensor& x, const Tensor& wg, const Tensor& wu, const Optional& bg, const Optional& bu, const RowsOf& rows, int64_t act, Tensor* kept) {
     const int64_t F = wg.size(0);
     Tensor h = at::empty(with_last(x, F), x.options());
     if (kept && tgt_gated_linear_kept_bytes(rows.N, (int)rows.C, (int)F, dtype_code(x), (int)act) > 0) *kept = at::empty({rows.N, 2 * F}, x.options());
+    const int64_t nbytes = tgt_gated_linear_fwd_workspace_bytes(rows.N, (int)rows.C, (int)F, dtype_code(x));
+    const Tensor work = room(nbytes, x);
     check(tgt_gated_linear_fwd(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), ptr(bg), ptr(bu), rows.N, (int)rows.C, (int)F, dtype_code(x), (int)act, h.data_ptr(),
-                               kept && kept->defined() ? kept->data_ptr() : nullptr, stream_of(x)),
+                               kept ? at_of(*kept) : nullptr, at_of(work), nbytes, stream_of(x)),
           "tgt_gated_linear_fwd");
     return h;
 }
@@ -195,7 +200,6 @@ struct GatedLinear : public torch::autograd::Function<GatedLinear> {
         if (ctx->saved_data["dw"].toBool()) { dwg = at::empty_like(wg); dwu = at::empty_like(wu); }
         if (biases & 1) dbg = at::empty({F}, x.options());
         if (biases & 2) dbu = at::empty({F}, x.options());
-        auto at_of = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
         void *dW[2] = {at_of(dwg), at_of(dwu)}, *db[2] = {at_of(dbg), at_of(dbu)};
         const int64_t nbytes = tgt_gated_linear_bwd_workspace_bytes(N, (int)C, (int)F, dtype_code(x));
         Tensor ws = at::empty({nbytes}, x.options().dtype(at::kByte));
@@ -228,8 +232,10 @@ Tensor linear_act_forward(const Tensor& x, const Tensor& w, const Optional& b, c
     const int64_t F = w.size(0);
     Tensor y = at::empty(with_last(x, F), x.options());
     if (kept && tgt_linear_epilogue_kept_bytes(rows.N, (int)rows.C, (int)F, dtype_code(x), (int)act) > 0) *kept = at::empty({rows.N, F}, x.options());
+    const int64_t nbytes = tgt_linear_epilogue_fwd_workspace_bytes(rows.N, (int)rows.C, (int)F, dtype_code(x));
+    const Tensor work = room(nbytes, x);
     check(tgt_linear_epilogue_fwd(x.data_ptr(), w.data_ptr(), ptr(b), ptr(r), rows.N, (int)rows.C, (int)F, dtype_code(x), (int)act, y.data_ptr(),
-                                  kept && kept->defined() ? kept->data_ptr() : nullptr, stream_of(x)),
+                                  kept ? at_of(*kept) : nullptr, at_of(work), nbytes, stream_of(x)),
           "tgt_linear_epilogue_fwd");
     return y;
 }
@@ -263,7 +269,6 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
             if (want_b) db = at::empty({F}, x.options());
             const int64_t nbytes = tgt_linear_epilogue_bwd_workspace_bytes(N, (int)C, (int)F, dtype_code(x), (int)act);
             Tensor ws = at::empty({nbytes}, x.options().dtype(at::kByte));
-            auto at_of = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
             check(tgt_linear_epilogue_bwd(x.data_ptr(), w.data_ptr(), at_of(b), dy.data_ptr(), N, (int)C, (int)F, dtype_code(x), (int)act, at_of(kept), at_of(dx), at_of(dw),
                                           at_of(db), ws.data_ptr(), nbytes, stream_of(x)),
                   "tgt_linear_epilogue_bwd");
@@ -322,8 +327,10 @@ Tensor gated_linear_8bit(const Tensor& x, const Tensor& xs, const Tensor& wg, co
     Tensor x2 = x.contiguous(), xs2 = xs.contiguous(), g2 = wg.contiguous(), gs2 = gs.contiguous(), u2 = wu.contiguous(), us2 = us.contiguous();
     Optional b1 = compact(bg), b2 = compact(bu);
     Tensor h = at::empty(with_last(x, F), x.options().dtype(type));
+    const int64_t nbytes = tgt_gated_linear_8bit_workspace_bytes(rows.N, (int)rows.C, (int)F);
+    const Tensor work = room(nbytes, x);
     check(tgt_gated_linear_8bit_fwd(x2.data_ptr(), xs2.data_ptr<float>(), g2.data_ptr(), gs2.data_ptr<float>(), u2.data_ptr(), us2.data_ptr<float>(), ptr(b1), ptr(b2),
-                                    rows.N, (int)rows.C, (int)F, code, (int)act, h.data_ptr(), stream_of(x)),
+                                    rows.N, (int)rows.C, (int)F, code, (int)act, h.data_ptr(), at_of(work), nbytes, stream_of(x)),
           "tgt_gated_linear_8bit_fwd");
     return h;
 }
@@ -345,8 +352,10 @@ Tensor linear_act_8bit(const Tensor& x, const Tensor& xs, const Tensor& w, const
     Tensor x2 = x.contiguous(), xs2 = xs.contiguous(), w2 = w.contiguous(), ws2 = ws.contiguous();
     Optional b2 = compact(b), r2 = compact(r);
     Tensor y = at::empty(with_last(x, F), x.options().dtype(type));
+    const int64_t nbytes = tgt_linear_epilogue_8bit_workspace_bytes(rows.N, (int)rows.C, (int)F);
+    const Tensor work = room(nbytes, x);
     check(tgt_linear_epilogue_8bit_fwd(x2.data_ptr(), xs2.data_ptr<float>(), w2.data_ptr(), ws2.data_ptr<float>(), ptr(b2), ptr(r2), rows.N, (int)rows.C, (int)F, code,
-                                       (int)act, y.data_ptr(), stream_of(x)),
+                                       (int)act, y.data_ptr(), at_of(work), nbytes, stream_of(x)),
           "tgt_linear_epilogue_8bit_fwd");
     return y;
 }
