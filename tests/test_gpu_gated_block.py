@@ -191,6 +191,17 @@ def test_wider_ones(cuda, shape, dt):
         check_linear(x, w, b, r, None, "relu", {"y": T.linear_act(x, w, b, "relu", r)})
 
 
+# Small widths and many nodes: the kernels that hold a weight's columns, at the largest weights that they are given
+@pytest.mark.parametrize("shape", [(4100, 512, 512), (4097, 68, 1000), (16400, 1024, 60)])
+def test_small_widths_many_rows(cuda, shape):
+    N, K, F = shape
+    case = gated_case(N, K, F // 2, F32, "silu", True)
+    check_gated(*case, "silu", run_gated(*case, "silu"))
+    case = linear_case(N, K, F, F32, True, True)
+    for act in (None, "gelu"):
+        check_linear(*case, act, run_linear(*case, act))
+
+
 # Few tiles and a long contraction, cut in pieces whose sums are joined: rows and columns that end inside a tile or a piece of one, contractions that end inside
 # a step and that change from one weight to the other inside and at the border of a piece, operands at odd addresses
 @pytest.mark.parametrize("dt", [F32, BF16])

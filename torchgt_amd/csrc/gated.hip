@@ -759,15 +759,20 @@ Args forward_args(const Call& c) {
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 bool needs_du(int n, int act) { return n == 2 || act != TGT_ACT_NONE; }      // (else dy is the operand itself)
 int in16(int dtype) { return dtype == TGT_DTYPE_F32 ? 4 : 8; }      // elements in 16 bytes
-// Whether the kernels for small widths (gated_tiles.hip, linear_tiles.hip) are the faster ones: weights of up to a million values and, forward + backward in us,
-// those kernels / the tiles of 128 and 256:   float32   300 x 128 x 128 25 / 59    2000 x 1024 x 1024 166 / 275   64000 x 256 x 256 206 / 236
-//                                                       64000 x 512 x 512 868 / 800      16000 x 1024 x 1024 827 / 756
-//                                             bfloat16  2000 x 512 x 512 47 / 59       16000 x 256 x 512 60 / 72         64000 x 256 x 256 94 / 101
-//                                                       64000 x 512 x 512 307 / 187      16000 x 1024 x 1024 316 / 174
+// Whether the kernels for small widths (gated_tiles.hip, linear_tiles.hip) are the faster ones; forward and backward kernels in us, those / the tiles of 128 and
+// 256 rows, nodes x K x F, n weights:
+//   bfloat16   one, no activation   500 x 128 x 128 19 / 33    2000 x 256 x 256 27 / 39    500 x 512 x 512 42 / 33    2000 x 512 x 512 45 / 50    8000 x 256 x 1024 70 / 55
+//                                   32000 x 256 x 256 59 / 48
+//              two                  2000 x 128 x 128 33 / 49   2000 x 256 x 256 56 / 60    500 x 64 x 1024 64 / 47    2000 x 512 x 512 97 / 68
+//   float32    one, no activation   2000 x 256 x 256 40 / 60   500 x 512 x 512 64 / 60     8000 x 512 x 512 123 / 150
+//              two                  2000 x 64 x 64 31 / 69     500 x 256 x 256 83 / 65     8000 x 256 x 256 115 / 117  32000 x 64 x 1024 347 / 564   8000 x 512 x 512 294 / 255
+// and a long contraction is not formed again where it can be kept (gelu, 2000 x 1024 x 64: bfloat16 60 / 47, float32 105 / 70; 32000: 178 / 282)
 bool narrow(const Call& c) {
-    const double products = (double)c.N * c.K * c.F * c.n;
-    return (int64_t)c.K * c.F * c.n <= (1 << 20) && products <= (c.dtype == TGT_DTYPE_F32 ? 8.6e9 : 2.1e9) && c.K % in16(c.dtype) == 0 && aligned16(c.x) &&
-           aligned16(c.W[0]) && aligned16(c.W[1]);
+    const bool f32 = c.dtype == TGT_DTYPE_F32;
+    const int64_t values = (int64_t)c.K * c.F * c.n;
+    if (values > (f32 && c.N >= 4096 ? 1 << 18 : 1 << 16) || (double)c.N * values > (f32 ? 8.6e9 : 1.6e9)) return false;
+    if (needs_du(c.n, c.act) && c.K >= 512 && (!f32 || c.N < 16384)) return false;
+    return c.K % in16(c.dtype) == 0 && aligned16(c.x) && aligned16(c.W[0]) && aligned16(c.W[1]);
 }
 NarrowArgs narrow_args(const Call& c, const void* more) {
     NarrowArgs a{};
@@ -777,9 +782,9 @@ NarrowArgs narrow_args(const Call& c, const void* more) {
     return a;
 }
 
-// What a forward that will have a backward is asked to keep: the products themselves, where forming them again takes longer than writing and reading them.
-// us of the gradients formed again / kept and read (with what the forward takes longer), bf16 16384 rows of K to 4096: see the end of this file's
-// comments on k_kept_grad; about 4 K / 1.2e15 + 2e-12 s a value against 3e-12.
+// What a forward that will have a backward is asked to keep: the products themselves, where forming them again takes longer than writing and reading them
+// (16384 x K x 4096 gated bf16, us: the product again with the gradients behind it, K 1024 360; kept values read 155, written 45 more in the forward; a
+// product takes about 0.3 us a K here, so 512 is where both take the same; float32 0.9 us a K and twice the bytes, three parts' products: 128).
 bool keeps(const Call& c) { return needs_du(c.n, c.act) && c.N > 64 && !narrow(c) && c.K >= (c.dtype == TGT_DTYPE_F32 ? 128 : 512); }
 
 int forward(const Call& c, const void* residual, void* out, void* kept, Room room, hipStream_t st) {
