@@ -507,8 +507,11 @@ int tgt_gated_linear_fwd(const void* d_x, const void* d_Wg, const void* d_Wu, co
                          int in_features, int out_features, int dtype, int act, void* d_h, void* d_kept, void* d_workspace,
                          int64_t workspace_bytes, void* stream);
 int64_t tgt_gated_linear_fwd_workspace_bytes(int64_t N, int in_features, int out_features, int dtype);
-/* Bytes of what a forward had better keep for its backward (both products, [N, 2 out_features] of `dtype`, 16-byte aligned) as
- * d_kept; 0: nothing, the backward forms them again.  d_kept = NULL is always possible in a forward, and then in its backward. */
+/* Bytes of what a forward had better keep for its backward (what both products are, a row of each weight side by side) as
+ * d_kept, 16-byte aligned; 0: nothing, the backward forms them again.  d_kept = NULL is always possible in a forward, and then in
+ * its backward.  float32: [N, 2, out_features].  bfloat16: [N, 2, out_features to the next multiple of 4] two-byte elements, four
+ * values in eight bytes: 14 bits each (two's complement, from the lowest bit on) and in the top byte a float's exponent, that of the
+ * largest; a value is its 14 bits times 2^(exponent - 139).  Exponent 255: the top 14 bits of each float instead. */
 int64_t tgt_gated_linear_kept_bytes(int64_t N, int in_features, int out_features, int dtype, int act);
 /* The same on operands in 8 bits (OCP e4m3): a value is its code times the scale of its row of x or of a weight.
  * in_features: a multiple of 16, d_x and the weights on 16-byte boundaries or not.  Biases and h are of `dtype`. */
@@ -525,7 +528,7 @@ int64_t tgt_gated_linear_bwd_workspace_bytes(int64_t N, int in_features, int out
 int tgt_gated_linear_bwd(const void* d_x, const void* d_Wg, const void* d_Wu, const void* d_bg, const void* d_bu,
                          const void* d_dh, int64_t N, int in_features, int out_features, int dtype, int act, const void* d_kept,
                          void* d_dx, void* const* d_dW, void* const* d_db, void* d_workspace, int64_t workspace_bytes, void* stream);
-/* y = act(x W^T + b) + residual; residual [N, out_features] or NULL (its gradient is dy itself); d_kept as above, [N, out_features] */
+/* y = act(x W^T + b) + residual; residual [N, out_features] or NULL (its gradient is dy itself); d_kept as above, of one weight */
 int tgt_linear_epilogue_fwd(const void* d_x, const void* d_W, const void* d_b, const void* d_residual, int64_t N, int in_features,
                             int out_features, int dtype, int act, void* d_y, void* d_kept, void* d_workspace, int64_t workspace_bytes, void* stream);
 int64_t tgt_linear_epilogue_fwd_workspace_bytes(int64_t N, int in_features, int out_features, int dtype);

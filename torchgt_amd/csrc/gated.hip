@@ -58,6 +58,38 @@ __device__ __forceinline__ void exchange(uint2& first, uint2& second) {
     second = make_uint2(x[1], y[1]);
 }
 
+// Four neighbouring values for the backward in the room of four bf16: one exponent, that of the largest, and 14 bits each, off by at most 2^-13 of the
+// largest.  What the gradients are formed of would otherwise be rounded as coarsely as they are themselves (bf16, 16384 x 1024 x 4096: the gradients off by 0.0030 instead of
+// 0.0023; 0.0017 is their own last rounding).  Values below 2^-114 lose bits; beside an infinity or a NaN each has sign, exponent and 5 bits of its own.
+__device__ __forceinline__ uint2 pack_four(const float (&v)[4]) {
+    uint32_t b[4], m[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b[i] = __float_as_uint(v[i]);
+    const uint32_t top = max(max(b[0] & 0x7fffffffu, b[1] & 0x7fffffffu), max(b[2] & 0x7fffffffu, b[3] & 0x7fffffffu)), exponent = max(top >> 23, 13u);
+    if (__builtin_expect(exponent == 255, 0)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m[i] = (v[i] != v[i] ? b[i] | 0x400000u : b[i]) >> 18;
+    } else {
+        const float scale = __uint_as_float((266 - exponent) << 23), at = 12582912.f;      // (1.5 2^23: the sum's low bits are the rounded product)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m[i] = __float_as_uint(__builtin_amdgcn_fmed3f(__builtin_fmaf(v[i], scale, at), at - 8191.f, at + 8191.f)) & 0x3fffu;
+    }
+    return make_uint2(m[0] | m[1] << 14 | m[2] << 28, m[2] >> 4 | m[3] << 10 | exponent << 24);
+}
+__device__ __forceinline__ void unpack_four(uint2 p, float (&v)[4]) {
+    const uint32_t exponent = p.y >> 24, m[4] = {p.x << 18, p.x >> 14 << 18, p.x >> 28 << 18 | p.y << 22, p.y >> 10 << 18};      // from the highest bit on
+    if (__builtin_expect(exponent == 255, 0)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(m[i]);
+    } else {
+        const float scale = __uint_as_float((exponent - 12) << 23);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = (float)((int)m[i] >> 18) * scale;
+    }
+}
+// elements of a row of one weight's kept values
+template <typename O> __host__ __device__ __forceinline__ int64_t kept_width(int64_t F) { return sizeof(O) == 2 ? (F + 3) / 4 * 4 : F; }
+
 // What becomes of a tile's sums.  WHOLE: the tile lies inside the result and all rows are aligned to 16 bytes; what is read is then asked for before the
 // first value is formed, and 16-bit rows are read and written 16 bytes a lane, 64 in a row, by an exchange between the pieces (8 bytes a lane: 16 rows of 32 bytes an
 // instruction).
@@ -184,9 +216,27 @@ __device__ __forceinline__ void finish(const Args& a, int64_t p0, int64_t q0, un
                 put(reinterpret_cast<O*>(a.out[0]) + q * a.out_ld + p, o);
                 if constexpr (kKeeps) {
                     if (a.kept) {
-                        O* to = reinterpret_cast<O*>(a.kept) + q * (kBy * a.p_count) + p;
+                        const int64_t width = kept_width<O>(a.p_count);
+                        O* to = reinterpret_cast<O*>(a.kept) + q * (kBy * width) + p;
 #pragma unroll
-                        for (int w = 0; w < kBy; ++w) put(to + w * a.p_count, keep[w]);
+                        for (int w = 0; w < kBy; ++w, to += width) {
+                            if constexpr (sizeof(O) == 2) {
+                                uint2 f[kGroup];
+#pragma unroll
+                                for (int n = 0; n < kGroup; ++n) {
+                                    if constexpr (!WHOLE) {
+#pragma unroll
+                                        for (int e = 0; e < 4; ++e)
+                                            if (e >= left[i0 + n]) keep[w][n][e] = 0.f;
+                                    }
+                                    f[n] = pack_four(keep[w][n]);
+                                }
+                                if constexpr (kWide) {
+                                    exchange(f[0], f[kGroup - 1]);
+                                    *reinterpret_cast<u32x4*>(to + wide_col) = u32x4{f[0].x, f[0].y, f[kGroup - 1].x, f[kGroup - 1].y};
+                                } else if (WHOLE || left[i0] > 0) *reinterpret_cast<uint2*>(to + col) = f[0];
+                            } else put(to, keep[w]);
+                        }
                     }
                 }
                 if constexpr (GRAD && kPair) put(reinterpret_cast<O*>(a.out[1]) + q * a.out_ld + p, o2);
@@ -441,32 +491,56 @@ template <typename O> __global__ __launch_bounds__(256) void k_column_sums(const
     if (w == 0 && col < M) partial[blockIdx.y * M + col] = (part[0][c] + part[1][c]) + (part[2][c] + part[3][c]);
 }
 
-// dg = dh u act'(g), du = dh act(g) (one weight: du = dy act'(u)) from what the forward kept, [N, F] of each weight side by side, and the column sums of what is
+// dg = dh u act'(g), du = dh act(g) (one weight: du = dy act'(u)) from what the forward kept, a row of each weight side by side, and the column sums of what is
 // written: workgroup (256 vectors of columns, share of the rows) -> partial[share][TWO ? 2 F : F] (null: not wanted).  Bound by memory: 16384 x
-// 4096 bf16, 671 MB.
-template <typename O, bool TWO, int ACT, int VE>
+// 4096 bf16, 671 MB.  WHOLE: rows of whole vectors, aligned.
+template <typename O, int VE, bool WHOLE> __device__ __forceinline__ void read_kept(const O* p, int n, float (&v)[VE]) {
+    if constexpr (sizeof(O) == 2) {
+        uint2 packed[VE / 4];
+#pragma unroll
+        for (int i = 0; i < VE / 4; ++i) packed[i] = reinterpret_cast<const uint2*>(p)[i];
+#pragma unroll
+        for (int i = 0; i < VE / 4; ++i) {
+            float f[4];
+            unpack_four(packed[i], f);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[i * 4 + e] = f[e];
+        }
+    } else {
+        const Four<O> f = load4<O, WHOLE>(p, n);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = f.e[e];
+    }
+}
+template <typename O, bool TWO, int ACT, int VE, bool WHOLE>
 __global__ __launch_bounds__(256) void k_kept_grad(const O* __restrict__ kept, const O* __restrict__ dy, int64_t N, int64_t F, int64_t rows_each, O* __restrict__ du,
                                                    float* __restrict__ partial) {
-    constexpr int NW = TWO ? 2 : 1;
+    constexpr int NW = TWO ? 2 : 1, U = 4;      // rows in flight
     constexpr bool EXACT = sizeof(O) == 4;
+    static_assert(VE == 4 || WHOLE, "");
     struct alignas(VE * sizeof(O)) Some { O e[VE]; };
-    const int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * VE, r0 = blockIdx.y * rows_each, r1 = r0 + rows_each < N ? r0 + rows_each : N;
+    const int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * VE, r0 = blockIdx.y * rows_each, r1 = r0 + rows_each < N ? r0 + rows_each : N, width = kept_width<O>(F);
     if (c >= F) return;
+    const int left = WHOLE || F - c >= VE ? VE : (int)(F - c);
     float sums[NW][VE];
 #pragma unroll
     for (int w = 0; w < NW; ++w)
 #pragma unroll
         for (int e = 0; e < VE; ++e) sums[w][e] = 0.f;
-    constexpr int U = 4;      // rows in flight
     for (int64_t r = r0; r < r1; r += U) {
-        Some in[U][NW + 1];
         const int n = r1 - r < U ? (int)(r1 - r) : U;
+        struct { float k[NW][VE]; Some dy; } in[U];
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             const int64_t row = i < n ? r + i : r;
 #pragma unroll
-            for (int w = 0; w < NW; ++w) in[i][w] = *reinterpret_cast<const Some*>(kept + (row * NW + w) * F + c);
-            in[i][NW] = *reinterpret_cast<const Some*>(dy + row * F + c);
+            for (int w = 0; w < NW; ++w) read_kept<O, VE, WHOLE>(kept + (row * NW + w) * width + c, left, in[i].k[w]);
+            if constexpr (WHOLE) in[i].dy = *reinterpret_cast<const Some*>(dy + row * F + c);
+            else {
+                const Four<O> f = load4<O, false>(dy + row * F + c, left);
+#pragma unroll
+                for (int e = 0; e < VE; ++e) in[i].dy.e[e] = f.e[e];
+            }
         }
 #pragma unroll
         for (int i = 0; i < U; ++i) {
@@ -474,12 +548,12 @@ __global__ __launch_bounds__(256) void k_kept_grad(const O* __restrict__ kept, c
             Some out[NW];
 #pragma unroll
             for (int e = 0; e < VE; ++e) {
-                const float g = to_float(in[i][0].e[e]), d = to_float(in[i][NW].e[e]);
+                const float g = in[i].k[0][e], d = to_float(in[i].dy.e[e]);
                 float o[NW];
                 if constexpr (TWO) {
                     float f, s;
                     act_and_slope<EXACT, ACT>(g, f, s);
-                    o[0] = d * to_float(in[i][1].e[e]) * s;
+                    o[0] = d * in[i].k[NW - 1][e] * s;
                     o[NW - 1] = d * f;
                 } else o[0] = slope_of<EXACT, ACT>(g, d);
 #pragma unroll
@@ -489,18 +563,27 @@ __global__ __launch_bounds__(256) void k_kept_grad(const O* __restrict__ kept, c
                 }
             }
 #pragma unroll
-            for (int w = 0; w < NW; ++w) *reinterpret_cast<Some*>(du + ((r + i) * NW + w) * F + c) = out[w];
+            for (int w = 0; w < NW; ++w) {
+                O* to = du + ((r + i) * NW + w) * F + c;
+                if constexpr (WHOLE) *reinterpret_cast<Some*>(to) = out[w];
+                else {
+#pragma unroll
+                    for (int e = 0; e < VE; ++e)
+                        if (e < left) to[e] = out[w].e[e];
+                }
+            }
         }
     }
     if (!partial) return;
 #pragma unroll
     for (int w = 0; w < NW; ++w)
 #pragma unroll
-        for (int e = 0; e < VE; ++e) partial[((int64_t)blockIdx.y * NW + w) * F + c + e] = sums[w][e];
+        for (int e = 0; e < VE; ++e)
+            if (WHOLE || e < left) partial[((int64_t)blockIdx.y * NW + w) * F + c + e] = sums[w][e];
 }
-template <typename O, bool TWO, int VE> void launch_kept_grad_as(const void* kept, const void* dy, int64_t N, int64_t F, int64_t rows_each, int shares, int act, void* du, float* partial, hipStream_t st) {
+template <typename O, bool TWO, int VE, bool WHOLE> void launch_kept_grad_as(const void* kept, const void* dy, int64_t N, int64_t F, int64_t rows_each, int shares, int act, void* du, float* partial, hipStream_t st) {
     const dim3 grid((unsigned)((F + 256 * VE - 1) / (256 * VE)), (unsigned)shares);
-#define X(ACT) hipLaunchKernelGGL((k_kept_grad<O, TWO, ACT, VE>), grid, dim3(256), 0, st, (const O*)kept, (const O*)dy, N, F, rows_each, (O*)du, partial)
+#define X(ACT) hipLaunchKernelGGL((k_kept_grad<O, TWO, ACT, VE, WHOLE>), grid, dim3(256), 0, st, (const O*)kept, (const O*)dy, N, F, rows_each, (O*)du, partial)
     switch (act) {
         case TGT_ACT_SILU: X(TGT_ACT_SILU); break;
         case TGT_ACT_GELU: X(TGT_ACT_GELU); break;
@@ -511,9 +594,9 @@ template <typename O, bool TWO, int VE> void launch_kept_grad_as(const void* kep
 }
 template <typename O> void launch_kept_grad(const void* kept, const void* dy, int n, int64_t N, int64_t F, int64_t rows_each, int shares, int act, void* du, float* partial, hipStream_t st) {
     constexpr int VE = 16 / (int)sizeof(O);
-    const bool whole = F % VE == 0 && (((uintptr_t)kept | (uintptr_t)dy | (uintptr_t)du) & 15) == 0;
-    if (n == 2) return whole ? launch_kept_grad_as<O, true, VE>(kept, dy, N, F, rows_each, shares, act, du, partial, st) : launch_kept_grad_as<O, true, 1>(kept, dy, N, F, rows_each, shares, act, du, partial, st);
-    return whole ? launch_kept_grad_as<O, false, VE>(kept, dy, N, F, rows_each, shares, act, du, partial, st) : launch_kept_grad_as<O, false, 1>(kept, dy, N, F, rows_each, shares, act, du, partial, st);
+    const bool whole = F % VE == 0 && (((uintptr_t)dy | (uintptr_t)du) & 15) == 0;
+    if (n == 2) return whole ? launch_kept_grad_as<O, true, VE, true>(kept, dy, N, F, rows_each, shares, act, du, partial, st) : launch_kept_grad_as<O, true, 4, false>(kept, dy, N, F, rows_each, shares, act, du, partial, st);
+    return whole ? launch_kept_grad_as<O, false, VE, true>(kept, dy, N, F, rows_each, shares, act, du, partial, st) : launch_kept_grad_as<O, false, 4, false>(kept, dy, N, F, rows_each, shares, act, du, partial, st);
 }
 
 // Rows F .. Fp - 1 of a weight are zeros
@@ -791,6 +874,7 @@ int forward(const Call& c, const void* residual, void* out, void* kept, Room roo
     int rc = check_call(c);
     if (rc != TGT_OK || c.N == 0) return rc;
     if (!out) { set_error("%s: null pointer", c.who); return TGT_ERR_INVALID_ARG; }
+    if (!aligned16(kept)) { set_error("%s: what is kept has to start on 16 bytes", c.who); return TGT_ERR_INVALID_ARG; }
     if (c.N > 64 && narrow(c) && !kept) {
         NarrowArgs a = narrow_args(c, residual);
         a.out[0] = out;
@@ -918,6 +1002,7 @@ int backward(const Call& c, const void* kept, const void* dy, void* dx, void* co
         return TGT_OK;
     }
     if (!dy) { set_error("%s: null pointer", c.who); return TGT_ERR_INVALID_ARG; }
+    if (!aligned16(kept)) { set_error("%s: what is kept has to start on 16 bytes", c.who); return TGT_ERR_INVALID_ARG; }
     const Plan p = plan_of(c.n, c.N, c.K, c.F, c.dtype, c.act);
     const int64_t need = workspace_bytes_of(c.n, c.N, c.K, c.F, c.dtype, c.act);
     if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)) {
@@ -1005,10 +1090,11 @@ int backward(const Call& c, const void* kept, const void* dy, void* dx, void* co
     return TGT_OK;
 }
 
+int64_t kept_room(int n, int64_t N, int F, int dtype) { return N * n * (dtype == TGT_DTYPE_F32 ? kept_width<float>(F) * 4 : kept_width<b16>(F) * 2); }
 int64_t kept_bytes_of(int n, int64_t N, int K, int F, int dtype, int act) {
     if (N < 0 || K < 1 || F < 1 || (dtype != TGT_DTYPE_F32 && dtype != TGT_DTYPE_BF16)) return -1;
     const Call c{"", nullptr, {nullptr, nullptr}, {nullptr, nullptr}, n, N, K, F, dtype, act};
-    return keeps(c) ? N * n * F * (dtype == TGT_DTYPE_F32 ? 4 : 2) : 0;
+    return keeps(c) ? kept_room(n, N, F, dtype) : 0;
 }
 int64_t fwd_bytes_of(int n, int64_t N, int K, int F, int dtype, bool bits8) {
     if (N < 0 || K < 1 || F < 1 || (dtype != TGT_DTYPE_F32 && dtype != TGT_DTYPE_BF16)) return -1;

@@ -167,7 +167,7 @@ void* at_of(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor gated_forward(const Tensor& x, const Tensor& wg, const Tensor& wu, const Optional& bg, const Optional& bu, const RowsOf& rows, int64_t act, Tensor* kept) {
     const int64_t F = wg.size(0);
     Tensor h = at::empty(with_last(x, F), x.options());
-    if (kept && tgt_gated_linear_kept_bytes(rows.N, (int)rows.C, (int)F, dtype_code(x), (int)act) > 0) *kept = at::empty({rows.N, 2 * F}, x.options());
+    if (kept) *kept = room(tgt_gated_linear_kept_bytes(rows.N, (int)rows.C, (int)F, dtype_code(x), (int)act), x);
     const int64_t nbytes = tgt_gated_linear_fwd_workspace_bytes(rows.N, (int)rows.C, (int)F, dtype_code(x));
     const Tensor work = room(nbytes, x);
     check(tgt_gated_linear_fwd(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), ptr(bg), ptr(bu), rows.N, (int)rows.C, (int)F, dtype_code(x), (int)act, h.data_ptr(),
@@ -231,7 +231,7 @@ Tensor gated_linear(const Tensor& x, const Tensor& wg, const Tensor& wu, const O
 Tensor linear_act_forward(const Tensor& x, const Tensor& w, const Optional& b, const Optional& r, const RowsOf& rows, int64_t act, Tensor* kept) {
     const int64_t F = w.size(0);
     Tensor y = at::empty(with_last(x, F), x.options());
-    if (kept && tgt_linear_epilogue_kept_bytes(rows.N, (int)rows.C, (int)F, dtype_code(x), (int)act) > 0) *kept = at::empty({rows.N, F}, x.options());
+    if (kept) *kept = room(tgt_linear_epilogue_kept_bytes(rows.N, (int)rows.C, (int)F, dtype_code(x), (int)act), x);
     const int64_t nbytes = tgt_linear_epilogue_fwd_workspace_bytes(rows.N, (int)rows.C, (int)F, dtype_code(x));
     const Tensor work = room(nbytes, x);
     check(tgt_linear_epilogue_fwd(x.data_ptr(), w.data_ptr(), ptr(b), ptr(r), rows.N, (int)rows.C, (int)F, dtype_code(x), (int)act, y.data_ptr(),
