@@ -295,6 +295,19 @@ def test_gated_linear_other_activations(cuda, dt, act):
     check_gated(*case, act, run_gated(*case, act))
 
 
+# A stretch of the contraction for each half or quarter of a matrix instruction's rows, row blocks of 16 and 32, contractions and columns that end inside them
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("rows", [1, 3, 4, 5, 8, 9, 20, 40, 64])
+@pytest.mark.parametrize("shape", [(4096, 70), (2056, 1030), (1023, 13), (5000, 2050)])
+def test_few_rows_of_long_contractions(cuda, dt, rows, shape):
+    K, F = shape
+    x, wg, wu, bg, bu, _ = gated_case(rows, K, F, dt, "silu", True)
+    with torch.no_grad():
+        check_gated(x, wg, wu, bg, bu, None, "silu", {"h": T.gated_linear(x, wg, wu, bg, bu)})
+        x, w, b, r, _ = linear_case(rows, K, F, dt, True, True)
+        check_linear(x, w, b, r, None, "gelu", {"y": T.linear_act(x, w, b, "gelu", r)})
+
+
 @pytest.mark.parametrize("dt", [F32, BF16])
 @pytest.mark.parametrize("rows", [1, 2, 7, 15, 16, 17, 31, 32, 33, 64])
 @pytest.mark.parametrize("shape", [(64, 96), (1024, 200), (2000, 33), (77, 130)])
@@ -534,7 +547,7 @@ def test_quantize_rows_is_exact(cuda, dt):
 # ---- operands in 8 bits -------------------------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("out", [F32, BF16])
-@pytest.mark.parametrize("shape", [(1, 16, 1), (1, 1024, 96), (7, 64, 33), (17, 48, 130), (130, 128, 64), (300, 272, 140), (64, 4096, 100), (200, 4096, 130), (300, 1040, 520), (65, 2048, 264)])
+@pytest.mark.parametrize("shape", [(1, 16, 1), (1, 1024, 96), (7, 64, 33), (17, 48, 130), (130, 128, 64), (300, 272, 140), (64, 4096, 100), (3, 4096, 70), (7, 2064, 1030), (40, 4096, 70), (200, 4096, 130), (300, 1040, 520), (65, 2048, 264)])
 def test_products_in_8_bits(cuda, out, shape):
     N, K, F = shape
     g = torch.Generator().manual_seed(K + F)

@@ -27,13 +27,13 @@ def test_entry_points_refuse_bad_arguments():
     assert L.tgt_linear_epilogue_8bit_fwd(p, None, p, p, None, None, 4, 32, 8, 0, 0, p, None, 0, None) == BAD
     assert L.tgt_gated_linear_8bit_fwd(p, p, p, p, p, None, None, None, 4, 32, 8, 0, 0, p, None, 0, None) == BAD
     for fwd, lead in (("tgt_gated_linear", (p, p, p, None, None)), ("tgt_linear_epilogue", (p, p, None, None))):      # few rows, a long contraction: cut in pieces
-        need = getattr(L, fwd + "_fwd_workspace_bytes")(100, 4096, 512, 1)
+        need = getattr(L, fwd + "_fwd_workspace_bytes")(300, 4096, 512, 1)
         assert need > 0 and getattr(L, fwd + "_fwd_workspace_bytes")(64, 4096, 512, 1) == 0 == getattr(L, fwd + "_fwd_workspace_bytes")(0, 4096, 512, 1)
         assert getattr(L, fwd + "_fwd_workspace_bytes")(-1, 4096, 512, 1) == -1 and getattr(L, fwd + "_8bit_workspace_bytes")(5, 0, 512) == -1
         call = getattr(L, fwd + "_fwd")
-        assert call(*lead, 100, 4096, 512, 1, 3, p, None, p, 1024, None) == WORKSPACE and call(*lead, 100, 4096, 512, 1, 3, p, None, None, need, None) == WORKSPACE
-        assert call(*lead, 100, 4096, 512, 1, 3, p, None, ctypes.c_void_p(4100), need, None) == WORKSPACE
-    assert L.tgt_linear_epilogue_8bit_fwd(p, p, p, p, None, None, 100, 4096, 512, 1, 0, p, None, 0, None) == WORKSPACE
+        assert call(*lead, 300, 4096, 512, 1, 3, p, None, p, 1024, None) == WORKSPACE and call(*lead, 300, 4096, 512, 1, 3, p, None, None, need, None) == WORKSPACE
+        assert call(*lead, 300, 4096, 512, 1, 3, p, None, ctypes.c_void_p(4100), need, None) == WORKSPACE
+    assert L.tgt_linear_epilogue_8bit_fwd(p, p, p, p, None, None, 300, 4096, 512, 1, 0, p, None, 0, None) == WORKSPACE
     dW = (ctypes.c_void_p * 2)(4096, None)
     assert L.tgt_gated_linear_bwd(p, p, p, None, None, p, 4, 8, 8, 0, 3, None, p, dW, None, p, 1 << 20, None) == BAD      # one weight's gradient
     assert L.tgt_gated_linear_bwd(p, p, p, None, None, None, 4, 8, 8, 0, 3, None, p, None, None, p, 1 << 20, None) == BAD

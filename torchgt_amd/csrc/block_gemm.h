@@ -273,7 +273,7 @@ template <int FORM> __device__ __forceinline__ float again(const Args& a, int wh
 
 // Tile shape: COLS x ROWS of the result by WP x WQ waves
 template <int COLS, int ROWS, int WP_, int WQ_> struct Shape {
-    static constexpr int kCols = COLS, kRows = ROWS, WP = WP_, WQ = WQ_, kThreads = 64 * WP * WQ;
+    static constexpr int kCols = COLS, kRows = ROWS, WP = WP_, WQ = WQ_, kThreads = 64 * WP * WQ, kUsed = 16;
     static constexpr int FP = COLS / WP / 16, FQ = ROWS / WQ / 16;      // 16 x 16 pieces of a wave
     // which 16 columns / rows of the tile a wave's piece is
     static constexpr __host__ __device__ __forceinline__ int p_piece(int wave, int i) { return wave % WP * FP + i; }
@@ -433,7 +433,7 @@ __device__ __forceinline__ bool tile_of(const Args& a, unsigned splits, unsigned
 // A contraction that ends inside a step: what is left of it goes through registers, zeros behind its end.
 
 template <int PH_> struct Wide {
-    static constexpr int PH = PH_, kCols = 128 * PH, kRows = 256, kThreads = 512, FP = 4 * PH, FQ = 4;
+    static constexpr int PH = PH_, kCols = 128 * PH, kRows = 256, kThreads = 512, FP = 4 * PH, FQ = 4, kUsed = 16;
     static constexpr int kHalf = 128 * 128, kOperand = PH * kHalf, kStage = kOperand + 2 * kHalf, kStages = PH == 2 ? 2 : 3, kLds = kStages * kStage;
     // waves 0-3 and 4-7 have 64 columns of each half of P, a wave 32 rows of each half of Q
     static constexpr __host__ __device__ __forceinline__ int p_piece(int wave, int i) { return (i >> 2) * 8 + (wave >> 2) * 4 + (i & 3); }

@@ -110,6 +110,7 @@ __device__ __forceinline__ void finish(const Args& a, int64_t p0, int64_t q0, un
     for (int i = 0; i < kOut; ++i) {
         const int64_t n = a.p_count - (p0 + S::p_piece(wave, i * kBy) / kBy * 16 + col);
         left[i] = n < 4 ? (int)n : 4;
+        if (S::kUsed < 16 && col >= S::kUsed) left[i] = 0;
     }
     Four<O> in[kReads ? kOut : 1][S::FQ];
     if (kReads && more) {
@@ -248,7 +249,7 @@ template <typename T, typename O, int FORM, bool TWO, bool GRAD, typename S>
 __device__ __forceinline__ void epilogue(const Args& a, int64_t p0, int64_t q0, unsigned split, const f32x4 (&acc)[S::FP][S::FQ]) {
     constexpr int kCols = FORM == kForward && TWO ? S::kCols / 2 : S::kCols;
     const void* more = GRAD ? a.dy : a.residual;
-    const bool whole = p0 + kCols <= a.p_count && q0 + S::kRows <= a.q_count &&
+    const bool whole = S::kUsed == 16 && p0 + kCols <= a.p_count && q0 + S::kRows <= a.q_count &&
                        (FORM == kWeightGrad && a.partial ? sixteens<float>(a.partial, a.p_count) : sixteens<O>(a.out[0], a.out_ld) && sixteens<O>(a.out[1], a.out_ld)) &&
                        (!more || sixteens<O>(more, a.p_count)) && sixteens<O>(a.kept, a.p_count);
 #define X(ACT) do { if (whole) finish<T, O, FORM, TWO, GRAD, S, ACT, true>(a, p0, q0, split, acc); else finish<T, O, FORM, TWO, GRAD, S, ACT, false>(a, p0, q0, split, acc); } while (0)
@@ -329,7 +330,7 @@ __global__ __launch_bounds__(S::kThreads, 2) void k_wide(const Args a, const uns
 
 // The splits' sums of a tile S, added in their order, and what becomes of them: two pieces of columns and one of rows of each wave to a workgroup.
 template <typename S> struct Part {
-    static constexpr int kThreads = S::kThreads, FP = 2, FQ = 1, kLast = S::kThreads / 64 - 1;
+    static constexpr int kThreads = S::kThreads, kUsed = 16, FP = 2, FQ = 1, kLast = S::kThreads / 64 - 1;
     static constexpr int kParts = S::FQ * S::FP / 2;
     static __device__ __forceinline__ int p_piece(int wave, int i) { return S::p_piece(wave, i); }
     static __device__ __forceinline__ int q_piece(int wave, int) { return S::q_piece(wave, 0); }
@@ -360,36 +361,43 @@ __global__ __launch_bounds__(S::kThreads) void k_join(const Args a, const unsign
 // from memory to the matrix instructions without LDS, and the waves' sums are added in their order.  A wave asks for U steps of both operands at once;
 // with 16 waves that is 100 to 200 KB in flight on a CU.
 //   float32: v_mfma_f32_16x16x4_f32, products exact (a memory-bound kernel has no use for three parts)
-template <int BY, int NQ> struct FewShape {
-    static constexpr int kCols = 16 * BY, kRows = 16 * NQ, FP = BY, FQ = 1;
-    static __device__ __forceinline__ int p_piece(int, int i) { return i; }
-    static __device__ __forceinline__ int q_piece(int wave, int) { return wave; }
+//
+// Where 16 columns a workgroup leave CUs without one, a workgroup has 16 / NS columns, for up to 16 / NS rows: the 16 rows and columns of the matrix instruction are NS
+// stretches of the contraction beside each other, and only the products of a stretch with itself, the blocks on its diagonal, count.  7 x 4096 x 1024 bf16:
+// 9.4 us with 64 workgroups, 7.1 with 128; one row 7.3 with 64, 5.0 with 256.
+template <int BY, int NQ, int NS> struct FewShape {
+    static constexpr int kCols = 16 * BY, kRows = 16 * NQ, FP = BY, FQ = 1, kUsed = 16 / NS;
+    static constexpr __host__ __device__ __forceinline__ int p_piece(int, int i) { return i; }
+    static constexpr __host__ __device__ __forceinline__ int q_piece(int wave, int) { return wave; }
 };
-template <typename T, typename O, bool TWO, int NQ, bool ALIGNED>
+template <typename T, typename O, bool TWO, int NQ, int NS, bool ALIGNED>
 __global__ __launch_bounds__(1024) void k_few(const Args a) {
     constexpr int BY = TWO ? 2 : 1, CE = 16 / (int)sizeof(T), U = NQ == 4 ? 2 : 4;
-    using S = FewShape<BY, NQ>;
+    using S = FewShape<BY, NQ, NS>;
+    static_assert(NS == 1 || NQ == 1, "");
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, g = lane >> 4;
-    const int64_t p0 = (int64_t)blockIdx.x * 16;
-    const int64_t pr = p0 + (lane & 15) < a.p_count ? p0 + (lane & 15) : a.p_count - 1;
+    const int own = lane & (S::kUsed - 1), stretch = (lane & 15) / S::kUsed;
+    const int64_t p0 = (int64_t)blockIdx.x * S::kUsed, q0 = (int64_t)blockIdx.y * S::kRows;
+    const int64_t pr = p0 + own < a.p_count ? p0 + own : a.p_count - 1;
     const T *W[BY], *X[NQ];
 #pragma unroll
     for (int w = 0; w < BY; ++w) W[w] = reinterpret_cast<const T*>(a.P[w]) + pr * a.p_ld;
 #pragma unroll
     for (int j = 0; j < NQ; ++j) {
-        const int64_t q = 16 * j + (lane & 15) < a.q_count ? 16 * j + (lane & 15) : a.q_count - 1;
+        const int64_t q = q0 + 16 * j + own < a.q_count ? q0 + 16 * j + own : a.q_count - 1;
         X[j] = reinterpret_cast<const T*>(a.Q) + q * a.q_ld;
     }
     constexpr int kAtOnce = 4 * CE * U;      // contraction indices that a wave asks for at once
-    const int64_t each = (a.K + (int64_t)waves * kAtOnce - 1) / ((int64_t)waves * kAtOnce) * kAtOnce;
-    const int64_t k0 = wave * each, k1 = k0 + each < a.K ? k0 + each : a.K;
+    const int64_t each = (a.K + (int64_t)(waves * NS) * kAtOnce - 1) / ((int64_t)(waves * NS) * kAtOnce) * kAtOnce;
+    const int64_t first = wave * NS * each, k0 = first + stretch * each, k1 = k0 + each < a.K ? k0 + each : a.K;
     f32x4 acc[BY][NQ];
 #pragma unroll
     for (int w = 0; w < BY; ++w)
 #pragma unroll
         for (int j = 0; j < NQ; ++j) acc[w][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int64_t k = k0; k < k1; k += kAtOnce) {
+    for (int64_t done = 0; done < each && first + done < a.K; done += kAtOnce) {
+        const int64_t k = k0 + done;
         u32x4 wv[BY][U], xv[NQ][U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -439,9 +447,17 @@ __global__ __launch_bounds__(1024) void k_few(const Args a) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) t[e] += s[e];
         }
+        if constexpr (NS > 1) {      // to the first stretch's lanes
+            f32x4 all = t;
+#pragma unroll
+            for (int n = 1; n < NS; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) all[e] += __shfl(t[e], (lane + n * (S::kUsed / 4 * 16 + S::kUsed)) & 63);
+            t = all;
+        }
         total[w][0] = t;
     }
-    epilogue<T, O, kForward, TWO, false, S>(a, p0, 0, 0, total);
+    epilogue<T, O, kForward, TWO, false, S>(a, p0, q0, 0, total);
 }
 
 #if TGT_GATED_PART == 0
@@ -656,18 +672,22 @@ int launch_wide(Args a, int splits, hipStream_t st) {
     return TGT_OK;
 }
 
-template <typename T, typename O, bool TWO, int NQ, bool ALIGNED> int launch_few(const Args& a, hipStream_t st) {
-    constexpr int kBy = TWO ? 2 : 1, kAtOnce = 4 * (16 / (int)sizeof(T)) * (NQ == 4 ? 2 : 4);
+template <typename T, typename O, bool TWO, int NQ, int NS, bool ALIGNED> int launch_few(const Args& a, hipStream_t st) {
+    constexpr int kBy = TWO ? 2 : 1, kAtOnce = 4 * (16 / (int)sizeof(T)) * (NQ == 4 ? 2 : 4) * NS;
+    // halves of the columns while CUs are left without a workgroup and four waves have something to do
+    if constexpr (NQ == 1 && NS < 4) {
+        if (a.q_count <= 8 / NS && a.p_count * 2 * NS <= 16 * num_cus() && a.K >= 8 * kAtOnce) return launch_few<T, O, TWO, NQ, 2 * NS, ALIGNED>(a, st);
+    }
     // a share of the contraction for each wave, 4 (16 rows for each: so many lanes that add up) to 16 waves
     const int waves = (int)std::max<int64_t>(4, std::min<int64_t>(16, (a.K + kAtOnce - 1) / kAtOnce));
     const int bytes = waves * kBy * NQ * 64 * 16;      // at most 128 KB
-    auto* kernel = k_few<T, O, TWO, NQ, ALIGNED>;
+    auto* kernel = k_few<T, O, TWO, NQ, NS, ALIGNED>;
     if (16 * kBy * NQ * 64 * 16 > 65536) {
         static std::atomic<uint64_t> done{0};
         const int rc = allow_lds((const void*)kernel, 16 * kBy * NQ * 64 * 16, done);
         if (rc != TGT_OK) return rc;
     }
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((a.p_count + 15) / 16)), dim3(64 * waves), bytes, st, a);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((a.p_count + 16 / NS - 1) / (16 / NS)), (unsigned)((a.q_count + 16 * NQ - 1) / (16 * NQ))), dim3(64 * waves), bytes, st, a);
     TGT_HIP_CHECK(hipGetLastError());
     return TGT_OK;
 }
@@ -708,6 +728,9 @@ bool aligned16(const void* p, int64_t ld, int size) { return ((uintptr_t)p & 15)
 
 // One product in the form asked for; TWO: a.P[1] is given
 struct Room { void* p; int64_t bytes; };      // for the sums of splits
+// Whether a product is one of few rows: up to 64 of them, or not even a workgroup of 16 rows and 16 columns for every CU (us, kernel of few rows / tiles and
+// joined sums: 64 x 4096 x 1024 bf16 10.5 / 13.6, float32 18.3 / 23.8; 64 x 1024 x 4096 8.1 / 13.2; 65 x 1024 x 256 5.3 / 9.3)
+static inline bool few_rows(int64_t q_count, int64_t p_count) { return q_count <= 64 || (q_count + 15) / 16 * ((p_count + 15) / 16) <= num_cus(); }
 template <typename T, typename O> int product_forward(Args a, bool grad, Room room, hipStream_t st);
 template <typename T> int product_input_grad(Args a, Room room, hipStream_t st);
 template <typename T> int product_weight_grad(const Args& a, int splits, hipStream_t st);
@@ -732,8 +755,12 @@ template <typename T, typename O> int product_forward(Args a, bool grad, Room ro
     constexpr int kStages = sizeof(T) == 4 ? 1 : 2;
     const bool two = a.P[1] != nullptr;
     const bool al = aligned16(a.Q, a.q_ld, sizeof(T)) && aligned16(a.P[0], a.p_ld, sizeof(T)) && (!two || aligned16(a.P[1], a.p_ld, sizeof(T)));
-    if (!grad && a.q_count <= 64) {
-#define X(TWO, NQ, AL) if (two == TWO && a.q_count <= 16 * NQ && al == AL) return launch_few<T, O, TWO, NQ, AL>(a, st)
+    if (!grad && few_rows(a.q_count, a.p_count)) {
+        // more rows to a workgroup only where there is one for every CU: they share its reads of the weights, but a workgroup takes longer by 3 us for 16 rows of 4096
+        // (64 x 4096 x 1024 bf16, us: 16 rows each 10.5, all 64 20.8)
+        const int64_t blocks = (a.p_count + 15) / 16, sixteens = (a.q_count + 15) / 16;
+        const int nq = blocks * sixteens <= num_cus() ? 1 : blocks * ((sixteens + 1) / 2) <= num_cus() || sixteens <= 2 ? 2 : 4;
+#define X(TWO, NQ, AL) if (two == TWO && (nq == NQ || (NQ == 1 && sixteens == 1)) && al == AL) return launch_few<T, O, TWO, NQ, 1, AL>(a, st)
         X(false, 1, true); X(true, 1, true); X(false, 2, true); X(true, 2, true); X(false, 4, true); X(true, 4, true);
         X(false, 1, false); X(true, 1, false); X(false, 2, false); X(true, 2, false); X(false, 4, false); X(true, 4, false);
 #undef X
@@ -875,7 +902,7 @@ int forward(const Call& c, const void* residual, void* out, void* kept, Room roo
     if (rc != TGT_OK || c.N == 0) return rc;
     if (!out) { set_error("%s: null pointer", c.who); return TGT_ERR_INVALID_ARG; }
     if (!aligned16(kept)) { set_error("%s: what is kept has to start on 16 bytes", c.who); return TGT_ERR_INVALID_ARG; }
-    if (c.N > 64 && narrow(c) && !kept) {
+    if (!few_rows(c.N, c.F) && narrow(c) && !kept) {
         NarrowArgs a = narrow_args(c, residual);
         a.out[0] = out;
         KernelTimer t(KS_LINEAR_FWD, st);
@@ -1098,7 +1125,7 @@ int64_t kept_bytes_of(int n, int64_t N, int K, int F, int dtype, int act) {
 }
 int64_t fwd_bytes_of(int n, int64_t N, int K, int F, int dtype, bool bits8) {
     if (N < 0 || K < 1 || F < 1 || (dtype != TGT_DTYPE_F32 && dtype != TGT_DTYPE_BF16)) return -1;
-    if (N <= 64) return 0;
+    if (few_rows(N, F)) return 0;
     return bits8 ? room_of<e4m3>(F, N, K, n) : dtype == TGT_DTYPE_F32 ? room_of<float>(F, N, K, n) : room_of<b16>(F, N, K, n);
 }
 int64_t workspace_bytes_of(int n, int64_t N, int K, int F, int dtype, int act) {
