@@ -662,6 +662,33 @@ def test_infinities_and_nans_stay_in_their_rows(cuda, rows):
         assert torch.equal(gw.isinf().cpu(), wantw.isinf()) and torch.equal(gw.isnan().cpu(), wantw.isnan())
 
 
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_infinities_in_contractions_in_pieces(cuda, dt):
+    """The same where a contraction is cut in pieces: infinities in several pieces, of both weights of the input gradient."""
+    N, K, F = 300, 2048, 1032
+    x, w = torch.ones(N, K, device="cuda", dtype=dt), torch.full((F, K), 0.5, device="cuda", dtype=dt)
+    x[0, 5], x[1, 2000], x[2, 700], x[2, 1900], w[3, 1500], w[4, 9], w[4, 1999] = float("inf"), float("nan"), float("inf"), float("-inf"), float("-inf"), float("inf"), float("inf")
+    y, want = T.linear_act(x, w).double().cpu(), x.double().cpu() @ w.double().cpu().T
+    assert torch.equal(y.isnan(), want.isnan()) and torch.equal(y.isinf(), want.isinf()) and torch.equal(y[want.isfinite()], want[want.isfinite()])
+    N, K, F = 70, 264, 2048
+    x, wg = torch.full((N, K), 0.25, device="cuda", dtype=dt), torch.full((F, K), 0.125, device="cuda", dtype=dt)
+    dh = torch.ones(N, F, device="cuda", dtype=dt)
+    for at in ((), (5,), (2000,), (5, 2000), (1023, 1024)):
+        for which in (0, 1):
+            W = [wg.clone(), wg.clone()]
+            for k, f in enumerate(at):
+                dh[3] = 0
+                dh[4, f] = float("inf")
+                W[which][f, 7 + k] = float("inf")
+            xl, gl, ul = (t.clone().requires_grad_(True) for t in (x, *W))
+            dx = torch.autograd.grad(T.gated_linear(xl, gl, ul, activation="relu"), xl, dh)[0].double().cpu()
+            X, WG, WU, DH = d(x), d(W[0]), d(W[1]), d(dh)
+            g, u = X @ WG.T, X @ WU.T
+            want = (DH * u * (g > 0)) @ WG + (DH * g.clamp(min=0)) @ WU
+            assert torch.equal(dx.isnan(), want.isnan()) and torch.equal(dx.isinf(), want.isinf()), (at, which)
+            assert (dx - want).abs()[want.isfinite()].le(want.abs()[want.isfinite()] * (3 * half_step(dt) + sums(2 * F + K) * 3)).all()
+
+
 def test_norm_of_a_row_with_a_nan_and_of_zeros(cuda):
     for dt in (F32, BF16):
         x = torch.ones(5, 100, device="cuda", dtype=dt)

@@ -264,9 +264,10 @@ template <int FORM> __device__ __forceinline__ float again(const Args& a, int wh
     const int64_t qs = FORM == kWeightGrad ? a.q_ld : 1;
     const float* P = reinterpret_cast<const float*>(a.P[which]);
     if (FORM == kForward) return again(0.f, Q, qs, P + p * a.p_ld + k0, 1, k1 - k0);
-    if (FORM == kInputGrad && k1 > a.K_first) {      // (k0 is 0)
-        const float s = again(0.f, Q, 1, P + p, a.p_ld, a.K_first);
-        return again(s, Q + a.K_first, 1, reinterpret_cast<const float*>(a.P[1]) + p, a.p_ld, k1 - a.K_first);
+    if (FORM == kInputGrad && k1 > a.K_first) {
+        const float s = k0 < a.K_first ? again(0.f, Q, 1, P + k0 * a.p_ld + p, a.p_ld, a.K_first - k0) : 0.f;
+        const int64_t from = k0 < a.K_first ? a.K_first : k0;
+        return again(s, Q + (from - k0), 1, reinterpret_cast<const float*>(a.P[1]) + (from - a.K_first) * a.p_ld + p, a.p_ld, k1 - from);
     }
     return again(0.f, Q, qs, P + k0 * a.p_ld + p, a.p_ld, k1 - k0);
 }

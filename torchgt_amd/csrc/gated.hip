@@ -704,11 +704,11 @@ template <typename T> Way way_of(int64_t p_count, int64_t q_count, int64_t K, in
     for (int h = 0; h <= (wide ? kSize == 1 ? 1 : 2 : 0); ++h) {      // (8-bit operands beside 128 sums: no registers, and reloads from scratch wait for all loads)
         const int64_t cols = (h == 2 ? 256 : 128) / by, rows = h ? 256 : 128, tiles = (p_count + cols - 1) / cols * ((q_count + rows - 1) / rows);
         const int64_t most = cut && h < 2 ? std::min(cus / tiles, steps / 2) : 1;
-        for (int64_t s = 1; s == 1 || s <= most; ++s) {
+        for (int64_t s = 1;; s = std::min(most, s + (s + 1) / 2)) {      // (a dozen of them: this runs on the host in every call)
             const int64_t each = (steps + s - 1) / s, bytes = s > 1 ? s * tiles * rows * 128 * 4 : 0;
-            if ((steps + each - 1) / each != s) continue;
             const double us = (tiles * s + cus - 1) / cus * (kFixed[h] + each * kStep[h]) + (s > 1 ? 4. + bytes * .4e-6 : 0.);
-            if (us < least) { least = us; best = Way{h, (int)s, each * Kind<T>::kStep, bytes}; }
+            if (us < least && (steps + each - 1) / each == s) { least = us; best = Way{h, (int)s, each * Kind<T>::kStep, bytes}; }
+            if (s >= most) break;
         }
     }
     return best;
