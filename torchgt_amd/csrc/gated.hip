@@ -61,7 +61,8 @@ __device__ __forceinline__ void exchange(uint2& first, uint2& second) {
 // Four neighbouring values for the backward in the room of four bf16: one exponent, that of the largest, and 14 bits each, off by at most 2^-13 of the
 // largest.  What the gradients are formed of would otherwise be rounded as coarsely as they are themselves (bf16, 16384 x 1024 x 4096: the gradients off by 0.0030 instead of
 // 0.0023; 0.0017 is their own last rounding).  Values below 2^-114 lose bits; beside an infinity or a NaN each has sign, exponent and 5 bits of its own.
-__device__ __forceinline__ uint2 pack_four(const float (&v)[4]) {
+// SIGNS: none but zeros become zero (an activation with an edge there), off by less than a step then, 2^-12 of the largest.
+template <bool SIGNS> __device__ __forceinline__ uint2 pack_four(const float (&v)[4]) {
     uint32_t b[4], m[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) b[i] = __float_as_uint(v[i]);
@@ -73,6 +74,11 @@ __device__ __forceinline__ uint2 pack_four(const float (&v)[4]) {
         const float scale = __uint_as_float((266 - exponent) << 23), at = 12582912.f;      // (1.5 2^23: the sum's low bits are the rounded product)
 #pragma unroll
         for (int i = 0; i < 4; ++i) m[i] = __float_as_uint(__builtin_amdgcn_fmed3f(__builtin_fmaf(v[i], scale, at), at - 8191.f, at + 8191.f)) & 0x3fffu;
+        if constexpr (SIGNS) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (m[i] == 0 && v[i] != 0.f) m[i] = v[i] < 0.f ? 0x3fffu : 1u;
+        }
     }
     return make_uint2(m[0] | m[1] << 14 | m[2] << 28, m[2] >> 4 | m[3] << 10 | exponent << 24);
 }
@@ -230,7 +236,7 @@ __device__ __forceinline__ void finish(const Args& a, int64_t p0, int64_t q0, un
                                         for (int e = 0; e < 4; ++e)
                                             if (e >= left[i0 + n]) keep[w][n][e] = 0.f;
                                     }
-                                    f[n] = pack_four(keep[w][n]);
+                                    f[n] = pack_four<ACT == TGT_ACT_RELU>(keep[w][n]);
                                 }
                                 if constexpr (kWide) {
                                     exchange(f[0], f[kGroup - 1]);
