@@ -67,20 +67,20 @@ template <bool SIGNS> __device__ __forceinline__ uint2 pack_four(const float (&v
 #pragma unroll
     for (int i = 0; i < 4; ++i) b[i] = __float_as_uint(v[i]);
     const uint32_t top = max(max(b[0] & 0x7fffffffu, b[1] & 0x7fffffffu), max(b[2] & 0x7fffffffu, b[3] & 0x7fffffffu)), exponent = max(top >> 23, 13u);
+    const float scale = __uint_as_float((266 - exponent) << 23), at = 12582912.f;      // (1.5 2^23: the sum's low bits are the rounded product)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m[i] = __float_as_uint(__builtin_amdgcn_fmed3f(__builtin_fmaf(v[i], scale, at), at - 8191.f, at + 8191.f));
+    if constexpr (SIGNS) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (m[i] == __float_as_uint(at) && v[i] != 0.f) m[i] += v[i] < 0.f ? -1 : 1;
+    }
     if (__builtin_expect(exponent == 255, 0)) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) m[i] = (v[i] != v[i] ? b[i] | 0x400000u : b[i]) >> 18;
-    } else {
-        const float scale = __uint_as_float((266 - exponent) << 23), at = 12582912.f;      // (1.5 2^23: the sum's low bits are the rounded product)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) m[i] = __float_as_uint(__builtin_amdgcn_fmed3f(__builtin_fmaf(v[i], scale, at), at - 8191.f, at + 8191.f)) & 0x3fffu;
-        if constexpr (SIGNS) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (m[i] == 0 && v[i] != 0.f) m[i] = v[i] < 0.f ? 0x3fffu : 1u;
-        }
     }
-    return make_uint2(m[0] | m[1] << 14 | m[2] << 28, m[2] >> 4 | m[3] << 10 | exponent << 24);
+    const auto select = [](uint32_t mask, uint32_t x, uint32_t y) { return (x & mask) | (y & ~mask); };      // one instruction
+    return make_uint2(select(0x3fffu, m[0], select(0xfffffffu, m[1] << 14, m[2] << 28)), select(0x3ffu, m[2] >> 4, select(0xffffffu, m[3] << 10, exponent << 24)));
 }
 __device__ __forceinline__ void unpack_four(uint2 p, float (&v)[4]) {
     const uint32_t exponent = p.y >> 24, m[4] = {p.x << 18, p.x >> 14 << 18, p.x >> 28 << 18 | p.y << 22, p.y >> 10 << 18};      // from the highest bit on
@@ -514,49 +514,59 @@ template <typename O> __global__ __launch_bounds__(256) void k_column_sums(const
 }
 
 // dg = dh u act'(g), du = dh act(g) (one weight: du = dy act'(u)) from what the forward kept, a row of each weight side by side, and the column sums of what is
-// written: workgroup (256 vectors of columns, share of the rows) -> partial[share][TWO ? 2 F : F] (null: not wanted).  Bound by memory: 16384 x
-// 4096 bf16, 671 MB.  WHOLE: rows of whole vectors, aligned.
-template <typename O, int VE, bool WHOLE> __device__ __forceinline__ void read_kept(const O* p, int n, float (&v)[VE]) {
-    if constexpr (sizeof(O) == 2) {
-        uint2 packed[VE / 4];
-#pragma unroll
-        for (int i = 0; i < VE / 4; ++i) packed[i] = reinterpret_cast<const uint2*>(p)[i];
+// written: workgroup (256 vectors: `across` of columns, so many rows side by side, share of the rows) -> partial[share][TWO ? 2 F : F] (null: not wanted).  Bound by
+// memory: 16384 x 4096 bf16, 671 MB in 152 us.  WHOLE: rows of whole vectors, aligned.
+template <typename O, int VE> struct KeptPiece {      // as it is in memory until it is used
+    uint2 p[VE / 4];
+    template <bool WHOLE> __device__ __forceinline__ void read(const O* from, int) {
+        if constexpr (WHOLE && VE == 8) {
+            const u32x4 v = *reinterpret_cast<const u32x4*>(from);
+            p[0] = make_uint2(v.x, v.y);
+            p[VE / 4 - 1] = make_uint2(v.z, v.w);
+        } else p[0] = *reinterpret_cast<const uint2*>(from);
+    }
+    __device__ __forceinline__ void values(float (&v)[VE]) const {
 #pragma unroll
         for (int i = 0; i < VE / 4; ++i) {
             float f[4];
-            unpack_four(packed[i], f);
+            unpack_four(p[i], f);
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[i * 4 + e] = f[e];
         }
-    } else {
-        const Four<O> f = load4<O, WHOLE>(p, n);
+    }
+};
+template <> struct KeptPiece<float, 4> {
+    Four<float> f;
+    template <bool WHOLE> __device__ __forceinline__ void read(const float* from, int n) { f = load4<float, WHOLE>(from, n); }
+    __device__ __forceinline__ void values(float (&v)[4]) const {
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = f.e[e];
     }
-}
+};
 template <typename O, bool TWO, int ACT, int VE, bool WHOLE>
-__global__ __launch_bounds__(256) void k_kept_grad(const O* __restrict__ kept, const O* __restrict__ dy, int64_t N, int64_t F, int64_t rows_each, O* __restrict__ du,
-                                                   float* __restrict__ partial) {
+__global__ __launch_bounds__(256) void k_kept_grad(const O* __restrict__ kept, const O* __restrict__ dy, int64_t N, int64_t F, int64_t rows_each, int across,
+                                                   O* __restrict__ du, float* __restrict__ partial) {
     constexpr int NW = TWO ? 2 : 1, U = 4;      // rows in flight
     constexpr bool EXACT = sizeof(O) == 4;
     static_assert(VE == 4 || WHOLE, "");
     struct alignas(VE * sizeof(O)) Some { O e[VE]; };
-    const int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * VE, r0 = blockIdx.y * rows_each, r1 = r0 + rows_each < N ? r0 + rows_each : N, width = kept_width<O>(F);
-    if (c >= F) return;
-    const int left = WHOLE || F - c >= VE ? VE : (int)(F - c);
+    __shared__ float side[256 * VE];
+    const int tx = threadIdx.x & (across - 1), ty = threadIdx.x / across, beside = 256 / across;
+    const int64_t c = ((int64_t)blockIdx.x * across + tx) * VE, r0 = blockIdx.y * rows_each, r1 = r0 + rows_each < N ? r0 + rows_each : N, width = kept_width<O>(F);
+    const int left = c >= F ? 0 : WHOLE || F - c >= VE ? VE : (int)(F - c);
     float sums[NW][VE];
 #pragma unroll
     for (int w = 0; w < NW; ++w)
 #pragma unroll
         for (int e = 0; e < VE; ++e) sums[w][e] = 0.f;
-    for (int64_t r = r0; r < r1; r += U) {
-        const int n = r1 - r < U ? (int)(r1 - r) : U;
-        struct { float k[NW][VE]; Some dy; } in[U];
+    for (int64_t r = r0 + ty; r < r1 && left; r += U * beside) {
+        const int n = (r1 - r + beside - 1) / beside < U ? (int)((r1 - r + beside - 1) / beside) : U;
+        struct { KeptPiece<O, VE> k[NW]; Some dy; } in[U];
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-            const int64_t row = i < n ? r + i : r;
+            const int64_t row = i < n ? r + i * beside : r;
 #pragma unroll
-            for (int w = 0; w < NW; ++w) read_kept<O, VE, WHOLE>(kept + (row * NW + w) * width + c, left, in[i].k[w]);
+            for (int w = 0; w < NW; ++w) in[i].k[w].template read<WHOLE>(kept + (row * NW + w) * width + c, left);
             if constexpr (WHOLE) in[i].dy = *reinterpret_cast<const Some*>(dy + row * F + c);
             else {
                 const Four<O> f = load4<O, false>(dy + row * F + c, left);
@@ -568,14 +578,17 @@ __global__ __launch_bounds__(256) void k_kept_grad(const O* __restrict__ kept, c
         for (int i = 0; i < U; ++i) {
             if (i >= n) break;
             Some out[NW];
+            float k[NW][VE];
+#pragma unroll
+            for (int w = 0; w < NW; ++w) in[i].k[w].values(k[w]);
 #pragma unroll
             for (int e = 0; e < VE; ++e) {
-                const float g = in[i].k[0][e], d = to_float(in[i].dy.e[e]);
+                const float g = k[0][e], d = to_float(in[i].dy.e[e]);
                 float o[NW];
                 if constexpr (TWO) {
                     float f, s;
                     act_and_slope<EXACT, ACT>(g, f, s);
-                    o[0] = d * in[i].k[NW - 1][e] * s;
+                    o[0] = d * k[NW - 1][e] * s;
                     o[NW - 1] = d * f;
                 } else o[0] = slope_of<EXACT, ACT>(g, d);
 #pragma unroll
@@ -586,7 +599,7 @@ __global__ __launch_bounds__(256) void k_kept_grad(const O* __restrict__ kept, c
             }
 #pragma unroll
             for (int w = 0; w < NW; ++w) {
-                O* to = du + ((r + i) * NW + w) * F + c;
+                O* to = du + ((r + i * beside) * NW + w) * F + c;
                 if constexpr (WHOLE) *reinterpret_cast<Some*>(to) = out[w];
                 else {
 #pragma unroll
@@ -598,14 +611,31 @@ __global__ __launch_bounds__(256) void k_kept_grad(const O* __restrict__ kept, c
     }
     if (!partial) return;
 #pragma unroll
-    for (int w = 0; w < NW; ++w)
+    for (int w = 0; w < NW; ++w) {
+        if (beside > 1) {      // the rows side by side, in their order
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < VE; ++e) side[e * 256 + threadIdx.x] = sums[w][e];
+            __syncthreads();
+            if (ty) continue;
+#pragma unroll
+            for (int e = 0; e < VE; ++e)
+                for (int k = 1; k < beside; ++k) sums[w][e] += side[e * 256 + k * across + tx];
+        }
 #pragma unroll
         for (int e = 0; e < VE; ++e)
-            if (WHOLE || e < left) partial[((int64_t)blockIdx.y * NW + w) * F + c + e] = sums[w][e];
+            if (e < left) partial[((int64_t)blockIdx.y * NW + w) * F + c + e] = sums[w][e];
+    }
+}
+int across_of(int64_t F, int VE) {
+    int n = 1;
+    while (n < 256 && n * VE < F) n *= 2;
+    return n;
 }
 template <typename O, bool TWO, int VE, bool WHOLE> void launch_kept_grad_as(const void* kept, const void* dy, int64_t N, int64_t F, int64_t rows_each, int shares, int act, void* du, float* partial, hipStream_t st) {
-    const dim3 grid((unsigned)((F + 256 * VE - 1) / (256 * VE)), (unsigned)shares);
-#define X(ACT) hipLaunchKernelGGL((k_kept_grad<O, TWO, ACT, VE, WHOLE>), grid, dim3(256), 0, st, (const O*)kept, (const O*)dy, N, F, rows_each, (O*)du, partial)
+    const int across = across_of(F, VE);
+    const dim3 grid((unsigned)((F + across * VE - 1) / (across * VE)), (unsigned)shares);
+#define X(ACT) hipLaunchKernelGGL((k_kept_grad<O, TWO, ACT, VE, WHOLE>), grid, dim3(256), 0, st, (const O*)kept, (const O*)dy, N, F, rows_each, across, (O*)du, partial)
     switch (act) {
         case TGT_ACT_SILU: X(TGT_ACT_SILU); break;
         case TGT_ACT_GELU: X(TGT_ACT_GELU); break;
@@ -709,10 +739,10 @@ template <typename T> Way way_of(int64_t p_count, int64_t q_count, int64_t K, in
     double least = 1e300;
     for (int h = 0; h <= (wide ? kSize == 1 ? 1 : 2 : 0); ++h) {      // (8-bit operands beside 128 sums: no registers, and reloads from scratch wait for all loads)
         const int64_t cols = (h == 2 ? 256 : 128) / by, rows = h ? 256 : 128, tiles = (p_count + cols - 1) / cols * ((q_count + rows - 1) / rows);
-        const int64_t most = cut && h < 2 ? std::min(cus / tiles, steps / 2) : 1;
+        const int64_t slots = h ? cus : 2 * cus, most = cut && h < 2 ? std::min(slots / tiles, steps / 2) : 1;      // (two workgroups of the small tiles to a CU, a third slower each)
         for (int64_t s = 1;; s = std::min(most, s + (s + 1) / 2)) {      // (a dozen of them: this runs on the host in every call)
             const int64_t each = (steps + s - 1) / s, bytes = s > 1 ? s * tiles * rows * 128 * 4 : 0;
-            const double us = (tiles * s + cus - 1) / cus * (kFixed[h] + each * kStep[h]) + (s > 1 ? 4. + bytes * .4e-6 : 0.);
+            const double us = (tiles * s + slots - 1) / slots * (kFixed[h] + each * kStep[h] * (tiles * s > cus && !h ? 1.3 : 1.)) + (s > 1 ? 4. + bytes * .4e-6 : 0.);
             if (us < least && (steps + each - 1) / each == s) { least = us; best = Way{h, (int)s, each * Kind<T>::kStep, bytes}; }
             if (s >= most) break;
         }
@@ -720,14 +750,6 @@ template <typename T> Way way_of(int64_t p_count, int64_t q_count, int64_t K, in
     return best;
 }
 bool wide_rows(const Args& a) { return a.K >= 256 && a.p_ld < (1 << 21) && a.q_ld < (1 << 21); }
-// a tile of one half takes 0.59 of the time of one with two
-int wide_halves(const Args& a, int cols, int splits) {
-    if (!wide_rows(a)) return 0;
-    const int64_t high = (a.q_count + 255) / 256 * splits, cus = num_cus(), one = (a.p_count + cols - 1) / cols * high, two = (a.p_count + 2 * cols - 1) / (2 * cols) * high;
-    if (one < cus * 3 / 4) return 0;
-    return 100 * ((two + cus - 1) / cus) <= 59 * ((one + cus - 1) / cus) ? 2 : 1;
-}
-
 bool aligned16(const void* p, int64_t ld, int size) { return ((uintptr_t)p & 15) == 0 && ld * size % 16 == 0; }
 
 }  // namespace
@@ -739,7 +761,7 @@ struct Room { void* p; int64_t bytes; };      // for the sums of splits
 static inline bool few_rows(int64_t q_count, int64_t p_count) { return q_count <= 64 || (q_count + 15) / 16 * ((p_count + 15) / 16) <= num_cus(); }
 template <typename T, typename O> int product_forward(Args a, bool grad, Room room, hipStream_t st);
 template <typename T> int product_input_grad(Args a, Room room, hipStream_t st);
-template <typename T> int product_weight_grad(const Args& a, int splits, hipStream_t st);
+template <typename T> int product_weight_grad(Args a, int& splits, hipStream_t st);      // (more than one split: to a.partial)
 
 // Bytes that the sums of splits take, whatever the operands' alignment
 template <typename T> int64_t room_of(int64_t p_count, int64_t q_count, int64_t K, int by) {
@@ -803,26 +825,29 @@ template <typename T> int product_input_grad(Args a, Room room, hipStream_t st) 
 #undef X
     return TGT_ERR_INVALID_ARG;
 }
-template <typename T> int product_weight_grad(const Args& a, int splits, hipStream_t st) {
+template <typename T> int product_weight_grad(Args a, int& splits, hipStream_t st) {
     constexpr int kStages = sizeof(T) == 4 ? 1 : 2;
     const bool al = aligned16(a.Q, a.q_ld, sizeof(T)) && aligned16(a.P[0], a.p_ld, sizeof(T));
+    const Way way = way_of<T>(a.p_count, a.q_count, a.K, 1, sizeof(T) < 4 && al && wide_rows(a) && a.p_count % 8 == 0 && a.q_count % 8 == 0, true);
+    splits = way.splits;
+    a.K_each = way.K_each;
+    if (way.splits == 1) a.partial = nullptr;
     if constexpr (sizeof(T) < 4) {
-        const int halves = al && a.p_count % 8 == 0 && a.q_count % 8 == 0 ? wide_halves(a, 128, splits) : 0;
-        if (halves == 2) return launch_wide<T, T, kWeightGrad, false, false, Wide<2>>(a, splits, st);
-        if (halves == 1) return launch_wide<T, T, kWeightGrad, false, false, Wide<1>>(a, splits, st);
+        if (way.halves == 2) return launch_wide<T, T, kWeightGrad, false, false, Wide<2>>(a, way.splits, st);
+        if (way.halves == 1) return launch_wide<T, T, kWeightGrad, false, false, Wide<1>>(a, way.splits, st);
     }
-    if (al) return launch<T, T, kWeightGrad, false, false, true, Square, kStages>(a, splits, st);
-    return launch<T, T, kWeightGrad, false, false, false, Square, kStages>(a, splits, st);
+    if (al) return launch<T, T, kWeightGrad, false, false, true, Square, kStages>(a, way.splits, st);
+    return launch<T, T, kWeightGrad, false, false, false, Square, kStages>(a, way.splits, st);
 }
 #endif
 #if TGT_GATED_PART == 1
 template int product_forward<b16, b16>(Args, bool, Room, hipStream_t);
 template int product_input_grad<b16>(Args, Room, hipStream_t);
-template int product_weight_grad<b16>(const Args&, int, hipStream_t);
+template int product_weight_grad<b16>(Args, int&, hipStream_t);
 #elif TGT_GATED_PART == 2
 template int product_forward<float, float>(Args, bool, Room, hipStream_t);
 template int product_input_grad<float>(Args, Room, hipStream_t);
-template int product_weight_grad<float>(const Args&, int, hipStream_t);
+template int product_weight_grad<float>(Args, int&, hipStream_t);
 #elif TGT_GATED_PART == 3
 template int product_forward<e4m3, b16>(Args, bool, Room, hipStream_t);
 template int product_forward<e4m3, float>(Args, bool, Room, hipStream_t);
@@ -880,13 +905,13 @@ int in16(int dtype) { return dtype == TGT_DTYPE_F32 ? 4 : 8; }      // elements 
 //   bfloat16   one, no activation   500 x 128 x 128 19 / 33    2000 x 256 x 256 27 / 39    500 x 512 x 512 42 / 33    2000 x 512 x 512 45 / 50    8000 x 256 x 1024 70 / 55
 //                                   32000 x 256 x 256 59 / 48
 //              two                  2000 x 128 x 128 33 / 49   2000 x 256 x 256 56 / 60    500 x 64 x 1024 64 / 47    2000 x 512 x 512 97 / 68
-//   float32    one, no activation   2000 x 256 x 256 40 / 60   500 x 512 x 512 64 / 60     8000 x 512 x 512 123 / 150
+//   float32    one, no activation   2000 x 256 x 256 40 / 60   500 x 512 x 512 64 / 49     2000 x 512 x 512 72 / 89    8000 x 512 x 512 123 / 150
 //              two                  2000 x 64 x 64 31 / 69     500 x 256 x 256 83 / 65     8000 x 256 x 256 115 / 117  32000 x 64 x 1024 347 / 564   8000 x 512 x 512 294 / 255
 // and a long contraction is not formed again where it can be kept (gelu, 2000 x 1024 x 64: bfloat16 60 / 47, float32 105 / 70; 32000: 178 / 282)
 bool narrow(const Call& c) {
     const bool f32 = c.dtype == TGT_DTYPE_F32;
     const int64_t values = (int64_t)c.K * c.F * c.n;
-    if (values > (f32 && c.N >= 4096 ? 1 << 18 : 1 << 16) || (double)c.N * values > (f32 ? 8.6e9 : 1.6e9)) return false;
+    if (values > (f32 && c.N >= (needs_du(c.n, c.act) ? 4096 : 1024) ? 1 << 18 : 1 << 16) || (double)c.N * values > (f32 ? 8.6e9 : 1.6e9)) return false;
     if (needs_du(c.n, c.act) && c.K >= 512 && (!f32 || c.N < 16384)) return false;
     return c.K % in16(c.dtype) == 0 && aligned16(c.x) && aligned16(c.W[0]) && aligned16(c.W[1]);
 }
@@ -942,25 +967,20 @@ int forward_8bit(const Call& c, const float* x_scales, const float* s0, const fl
 
 // How the backward lays out its workspace, and how it cuts the nodes
 struct Plan {
-    int64_t du_bytes, between, bytes, K_each, rows_each;
-    int splits, shares, kept_shares;
+    int64_t du_bytes, between, bytes, rows_each;
+    int shares, kept_shares;
 };
 int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
 Plan plan_of(int n, int64_t N, int K, int F, int dtype, int act) {
     Plan p{};
     const int64_t size = dtype == TGT_DTYPE_F32 ? 4 : 2, cols = (int64_t)n * F;
-    const int step = dtype == TGT_DTYPE_F32 ? Kind<float>::kStep : Kind<b16>::kStep;
     p.du_bytes = n == 2 || act != TGT_ACT_NONE ? up16(N * cols * size) : 0;      // (without an activation dy is the operand itself)
-    // two workgroups per CU: fewer tiles than that are cut along the nodes, in pieces of eight steps at least
-    const int64_t tiles = ((cols + 127) / 128) * (((int64_t)K + 127) / 128);
-    const int64_t want = std::max<int64_t>(1, std::min<int64_t>((512 + tiles - 1) / tiles, (N + 8 * step - 1) / (8 * step)));
-    p.K_each = ((N + want - 1) / std::max<int64_t>(1, want) + step - 1) / step * step;
-    p.splits = N > 0 ? (int)((N + p.K_each - 1) / p.K_each) : 1;
     p.shares = (int)std::max<int64_t>(1, std::min<int64_t>(512, (N + 31) / 32));
     p.rows_each = (N + p.shares - 1) / p.shares;
-    p.kept_shares = (int)std::max<int64_t>(1, std::min<int64_t>(512, (N + 7) / 8));      // (their rows are in flight together: latency counts before bandwidth)
-    // one after the other: the sums of dx's splits, those of the weights' gradients
-    p.between = std::max(p.splits > 1 ? up16((int64_t)p.splits * cols * K * 4) : 0, dtype == TGT_DTYPE_F32 ? room_of<float>(K, N, cols, 1) : room_of<b16>(K, N, cols, 1));
+    const int beside = 256 / across_of(F, in16(dtype));
+    p.kept_shares = (int)std::max<int64_t>(1, std::min<int64_t>(512, (N + 8 * beside - 1) / (8 * beside)));      // (their rows are in flight together: latency counts before bandwidth)
+    // one after the other: the sums of dx's splits, those of the weights' gradients (no more than their whole tiles would take)
+    p.between = up16(dtype == TGT_DTYPE_F32 ? std::max(room_of<float>(K, N, cols, 1), room_of<float>(K, cols, N, 1)) : std::max(room_of<b16>(K, N, cols, 1), room_of<b16>(K, cols, N, 1)));
     p.bytes = p.du_bytes + p.between + up16((int64_t)p.kept_shares * cols * 4);
     return p;
 }
@@ -1084,26 +1104,27 @@ int backward(const Call& c, const void* kept, const void* dy, void* dx, void* co
         a.Q = du;
         a.p_ld = c.K; a.q_ld = cols;
         a.p_count = c.K; a.q_count = cols;
-        a.K = a.K_first = c.N; a.K_each = p.K_each;
+        a.K = a.K_first = c.N;
         a.out[0] = dW[0]; a.out[1] = c.n == 2 ? dW[1] : nullptr;
         a.q_first = c.F;
         a.out_ld = c.K;
-        a.partial = p.splits > 1 ? (float*)after : nullptr;
+        a.partial = (float*)after;
+        int splits = 1;
         KernelTimer t(KS_LINEAR_DW, st);
-        rc = f32 ? product_weight_grad<float>(a, p.splits, st) : product_weight_grad<b16>(a, p.splits, st);
+        rc = f32 ? product_weight_grad<float>(a, splits, st) : product_weight_grad<b16>(a, splits, st);
         if (rc != TGT_OK) return rc;
-        if (p.splits >= 16 && cols * c.K <= 65536) {      // few elements, many splits: 16 slices of the splits side by side
+        if (splits >= 16) {      // few elements, many splits: 16 slices of the splits side by side
             tgt_reduce_desc r{};
-            r.partial = a.partial; r.workers = p.splits; r.n = (int)(cols * c.K); r.n_out = c.n;
+            r.partial = a.partial; r.workers = splits; r.n = (int)(cols * c.K); r.n_out = c.n;
             r.out[0] = dW[0];
             if (c.n == 2) { r.out[1] = dW[1]; r.begin[1] = c.F * c.K; }
             rc = reduce_partials(&r, 1, c.dtype, st);
             if (rc != TGT_OK) return rc;
-        } else if (p.splits > 1) {
+        } else if (splits > 1) {
             const int64_t n = cols * c.K, first = (int64_t)c.F * c.K;
             const dim3 grid((unsigned)((n + 1023) / 1024));
-            if (f32) hipLaunchKernelGGL((k_add_splits<float>), grid, dim3(256), 0, st, a.partial, p.splits, n, first, (float*)dW[0], (float*)a.out[1]);
-            else hipLaunchKernelGGL((k_add_splits<b16>), grid, dim3(256), 0, st, a.partial, p.splits, n, first, (b16*)dW[0], (b16*)a.out[1]);
+            if (f32) hipLaunchKernelGGL((k_add_splits<float>), grid, dim3(256), 0, st, a.partial, splits, n, first, (float*)dW[0], (float*)a.out[1]);
+            else hipLaunchKernelGGL((k_add_splits<b16>), grid, dim3(256), 0, st, a.partial, splits, n, first, (b16*)dW[0], (b16*)a.out[1]);
             TGT_HIP_CHECK(hipGetLastError());
         }
     }
