@@ -514,7 +514,8 @@ int64_t tgt_gated_linear_fwd_workspace_bytes(int64_t N, int in_features, int out
  * largest; a value is its 14 bits times 2^(exponent - 139).  Exponent 255: the top 14 bits of each float instead. */
 int64_t tgt_gated_linear_kept_bytes(int64_t N, int in_features, int out_features, int dtype, int act);
 /* The same on operands in 8 bits (OCP e4m3): a value is its code times the scale of its row of x or of a weight.
- * in_features: a multiple of 16, d_x and the weights on 16-byte boundaries or not.  Biases and h are of `dtype`. */
+ * in_features: a multiple of 16, d_x and the weights on 16-byte boundaries or not.  Biases and h are of `dtype`.  Eight neighbouring
+ * products are added at a time, cut 13 binary places below the largest of them. */
 int tgt_gated_linear_8bit_fwd(const void* d_x, const float* d_x_scales, const void* d_Wg, const float* d_Wg_scales,
                               const void* d_Wu, const float* d_Wu_scales, const void* d_bg, const void* d_bu, int64_t N,
                               int in_features, int out_features, int dtype, int act, void* d_h, void* d_workspace, int64_t workspace_bytes,

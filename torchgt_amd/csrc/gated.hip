@@ -6,10 +6,13 @@
 // No counterpart in the reference, whose feed-forward block has one projection and a GELU (models/graphormer_dist_node_level.py:27-39).
 //
 // Backward.  With g = x Wg^T + bg, u = x Wu^T + bu:  dg = dh u act'(g), du = dh act(g);  dx = dg Wg + du Wu;  dWg = dg^T x, dWu = du^T x; biases: column
-// sums.  Where the contraction is long the forward keeps g and u (rounded to the tensors' type, like every activation of such a layer; h is formed of the
+// sums.  Where the contraction is long the forward keeps g and u (bfloat16: 14 bits and an exponent for four; h is formed of the
 // float32 values); where it is short they are not kept: a first kernel forms them again in float32.  Either writes dg and du, rounded to the tensors' type since
-// they are operands of the next two products; dx and dW are products of what it wrote.  dW over few output tiles is cut along the nodes, partial
-// sums in float32 added in a fixed order.
+// they are operands of the next two products; dx and dW are products of what it wrote.  A product of few output tiles is cut along its contraction, partial sums in float32 added in a fixed order.
+//
+// Measured (us; 2 n N K F operations and what a large library product of the same type reaches, 1422 TFLOP/s in bf16): gated 16384 x 1024 x 4096 bf16 forward
+// with kept values 300 to 333 (193; without kept values 266), kept gradients 149 (671 MB at 4.5 TB/s), input gradient 205 to 226 (193), weight gradients 238 to 262 (193):
+// a hot card is slower.  linear 16384 x 4096 x 1024: 114 to 129, 129 to 139, 136 to 146 (97 each).  8 bits, 4099 x 1024 x 2816 gated: 35 (18).
 #include "activations.h"
 #include "block_gemm.h"
 #include "gated_tiles.h"

