@@ -163,7 +163,7 @@ __device__ __forceinline__ void finish(const Args& a, int64_t p0, int64_t q0, un
 #pragma unroll
         for (int j = 0; j < S::FQ; ++j) {
             const int64_t q = q0 + S::q_piece(wave, j) * 16 + row;
-            if (!WHOLE && q >= a.q_count) continue;
+            if (!WHOLE && (q >= a.q_count || row >= S::kUsed)) continue;
             if constexpr (kWide && kReads) {
                 if (more) exchange(in[i0][j].v, in[i0 + 1][j].v);
             }
@@ -371,11 +371,11 @@ __global__ __launch_bounds__(S::kThreads) void k_join(const Args a, const unsign
 // with 16 waves that is 100 to 200 KB in flight on a CU.
 //   float32: v_mfma_f32_16x16x4_f32, products exact (a memory-bound kernel has no use for three parts)
 //
-// Where 16 columns a workgroup leave CUs without one, a workgroup has 16 / NS columns, for up to 16 / NS rows: the 16 rows and columns of the matrix instruction are NS
-// stretches of the contraction beside each other, and only the products of a stretch with itself, the blocks on its diagonal, count.  7 x 4096 x 1024 bf16:
-// 9.4 us with 64 workgroups, 7.1 with 128; one row 7.3 with 64, 5.0 with 256.
+// Where 16 columns and 16 rows a workgroup leave CUs without one, a workgroup has 16 / NS columns and as many rows: the 16 rows and columns of the matrix
+// instruction are NS stretches of the contraction beside each other, and only the products of a stretch with itself, the blocks on its diagonal, count.
+// x 4096 x 1024 bf16, us: one row 7.3 with 64 workgroups, 4.5 with 256; 7 rows 8.5 with 64, 6.1 with 128, 6.2 with 512; 16 rows 9.9 with 64, 6.5 with 256.
 template <int BY, int NQ, int NS> struct FewShape {
-    static constexpr int kCols = 16 * BY, kRows = 16 * NQ, FP = BY, FQ = 1, kUsed = 16 / NS;
+    static constexpr int kCols = 16 * BY, kRows = 16 * NQ / NS, FP = BY, FQ = 1, kUsed = 16 / NS;
     static constexpr __host__ __device__ __forceinline__ int p_piece(int, int i) { return i; }
     static constexpr __host__ __device__ __forceinline__ int q_piece(int wave, int) { return wave; }
 };
@@ -387,7 +387,7 @@ __global__ __launch_bounds__(1024) void k_few(const Args a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, g = lane >> 4;
     const int own = lane & (S::kUsed - 1), stretch = (lane & 15) / S::kUsed;
-    const int64_t p0 = (int64_t)blockIdx.x * S::kUsed, q0 = (int64_t)blockIdx.y * S::kRows;
+    const int64_t p0 = (int64_t)blockIdx.x * S::kUsed, q0 = (int64_t)blockIdx.y * S::kRows;      // (NS > 1: as many rows as columns)
     const int64_t pr = p0 + own < a.p_count ? p0 + own : a.p_count - 1;
     const T *W[BY], *X[NQ];
 #pragma unroll
@@ -715,7 +715,7 @@ template <typename T, typename O, bool TWO, int NQ, int NS, bool ALIGNED> int la
     constexpr int kBy = TWO ? 2 : 1, kAtOnce = 4 * (16 / (int)sizeof(T)) * (NQ == 4 ? 2 : 4) * NS;
     // halves of the columns while CUs are left without a workgroup and four waves have something to do
     if constexpr (NQ == 1 && NS < 4) {
-        if (a.q_count <= 8 / NS && a.p_count * 2 * NS <= 16 * num_cus() && a.K >= 8 * kAtOnce) return launch_few<T, O, TWO, NQ, 2 * NS, ALIGNED>(a, st);
+        if ((a.p_count * 2 * NS + 15) / 16 * ((a.q_count * 2 * NS + 15) / 16) <= num_cus() && a.K >= 8 * kAtOnce) return launch_few<T, O, TWO, NQ, 2 * NS, ALIGNED>(a, st);
     }
     // a share of the contraction for each wave, 4 (16 rows for each: so many lanes that add up) to 16 waves
     const int waves = (int)std::max<int64_t>(4, std::min<int64_t>(16, (a.K + kAtOnce - 1) / kAtOnce));
@@ -726,7 +726,7 @@ template <typename T, typename O, bool TWO, int NQ, int NS, bool ALIGNED> int la
         const int rc = allow_lds((const void*)kernel, 16 * kBy * NQ * 64 * 16, done);
         if (rc != TGT_OK) return rc;
     }
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((a.p_count + 16 / NS - 1) / (16 / NS)), (unsigned)((a.q_count + 16 * NQ - 1) / (16 * NQ))), dim3(64 * waves), bytes, st, a);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((a.p_count + 16 / NS - 1) / (16 / NS)), (unsigned)((a.q_count * NS + 16 * NQ - 1) / (16 * NQ))), dim3(64 * waves), bytes, st, a);
     TGT_HIP_CHECK(hipGetLastError());
     return TGT_OK;
 }
