@@ -654,11 +654,6 @@ template <typename O> void launch_kept_grad(const void* kept, const void* dy, in
     return whole ? launch_kept_grad_as<O, false, VE, true>(kept, dy, N, F, rows_each, shares, act, du, partial, st) : launch_kept_grad_as<O, false, 4, false>(kept, dy, N, F, rows_each, shares, act, du, partial, st);
 }
 
-// Rows F .. Fp - 1 of a weight are zeros
-template <typename O> __global__ __launch_bounds__(256) void k_pad_rows(const O* __restrict__ w, int64_t n, int64_t all, O* __restrict__ out) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) out[i] = i < n ? w[i] : O{};
-}
-
 __global__ __launch_bounds__(256) void k_zero(uint16_t* __restrict__ p, int64_t n) {
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = 0;
 }
@@ -1006,17 +1001,12 @@ int backward_narrow(const Call& c, const void* dy, void* dx, void* const* dW, vo
         NarrowArgs a = narrow_args(c, dy);
         for (int w = 0; w < c.n; ++w) { du[w] = a.out[w] = ws; ws += up16(c.N * Fp * size); }
         a.out_ld = Fp;
+        if (Fp != c.F) {      // (one weight: its rows behind the last are zeros for dx, their gradients are not wanted)
+            W[0] = a.padded = ws;
+            ws += up16((int64_t)Fp * c.K * size);
+        }
         KernelTimer t(KS_LINEAR_FWD, st);
         if (const int rc = gated_tiles(a, true, c.dtype, st)) return rc;
-    }
-    if (Fp != c.F) {      // (one weight: its rows behind the last are zeros for dx, their gradients are not wanted)
-        const int64_t n = (int64_t)c.F * c.K, all = (int64_t)Fp * c.K;
-        const dim3 grid((unsigned)std::min<int64_t>((all + 255) / 256, 1024));
-        if (f32) hipLaunchKernelGGL((k_pad_rows<float>), grid, dim3(256), 0, st, (const float*)c.W[0], n, all, (float*)ws);
-        else hipLaunchKernelGGL((k_pad_rows<b16>), grid, dim3(256), 0, st, (const b16*)c.W[0], n, all, (b16*)ws);
-        TGT_HIP_CHECK(hipGetLastError());
-        W[0] = ws;
-        ws += up16(all * size);
     }
     const bool want_w = dW && dW[0], want_b = db && (db[0] || (c.n == 2 && db[1]));
     const int64_t bytes = tgt_linear_bwd_workspace_bytes(c.n, c.K, Fp);

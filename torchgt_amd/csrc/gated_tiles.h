@@ -14,6 +14,7 @@ struct NarrowArgs {
     int K, F;
     int out_ld;             // F, or with `grad` F rounded up to 16 bytes: the columns behind F are zeros then
     int act;
+    void* padded;           // `grad` with one weight: where to put W[0] with rows of zeros up to out_ld (16-byte aligned), or null
 };
 
 // act(x W0^T + b0) * (x W1^T + b1), or with one weight act(x W0^T + b0) + residual; grad: the gradients of what the activation and the other factor

@@ -143,6 +143,14 @@ __global__ __launch_bounds__(kThreads, 2) void k_gated_tiles(const NarrowArgs a,
     const Rows rows((int64_t)blockIdx.x * kWaves + wave, a.N);
     const T* const x = reinterpret_cast<const T*>(a.x);
     const T* const more = reinterpret_cast<const T*>(a.more);
+    if constexpr (GRAD && !TWO) {
+        if (a.padded) {      // (a launch of its own costs more than the copy)
+            constexpr int VE = 16 / (int)sizeof(T);
+            const int all = (int)((int64_t)a.out_ld * a.K / VE), have = (int)((int64_t)a.F * a.K / VE), by = (int)(gridDim.x * gridDim.y) * kThreads;
+            for (int i = (int)(blockIdx.y * gridDim.x + blockIdx.x) * kThreads + (int)threadIdx.x; i < all; i += by)
+                reinterpret_cast<vec16*>(a.padded)[i] = i < have ? reinterpret_cast<const vec16*>(a.W[0])[i] : vec16{0u, 0u, 0u, 0u};
+        }
+    }
     Frags<P> f[RES ? RES : 1];
     Raw<T> raw;
     const auto operands = [&](Frags<P>& to) {
